@@ -582,4 +582,63 @@ struct SampleArgs {
 int sample_supported(int V, int H);
 void launch_sample_step(const SampleArgs& a, hipStream_t s);
 
+// gated linear recurrence (linrec.hip).  Sequences are [T, B, H] with unit stride along H and any
+// strides (in elements) along T and B; states are [B, H] contiguous fp32.
+constexpr int kLinrecSteps = 8;  // consecutive steps a wave holds in registers
+struct LinrecPlan {
+  int waves;          // waves of a workgroup; a tile is waves * kLinrecSteps steps
+  int tiles;          // tiles of the time axis
+  int segs, tiles_per_seg;  // segments of the time axis (1: no summary launch)
+};
+struct LinrecArgs {
+  const void *x, *f, *dh;      // inputs, gate pre-activations, output gradients (bf16 or fp32)
+  void *h, *dx, *df;           // outputs and gradients, same type
+  long x_t, x_b, f_t, f_b, dh_t, dh_b, h_t, h_b, dx_t, dx_b, df_t, df_b;
+  const float *h0, *dlast;     // optional (zeros)
+  float *hlast, *dh0;          // hlast: the state in place for the single step; dh0 optional
+  const int* lengths;          // optional [B], clamped to [0, T]
+  const unsigned char* starts; // optional [T, B], non-zero: the state restarts at this step
+  long starts_t, starts_b;
+  float* carry;                // [tiles, B, H] states in front of the tiles (forward: optional)
+  float *sumA, *sumB;          // [segs, B, H] segment pairs (segs > 1)
+  int T, B, H;
+  int tiles, tiles_per_seg, segs;  // set by the launcher
+};
+LinrecPlan linrec_plan(int T, int B, int H);
+void launch_linrec(LinrecArgs a, bool is_bf16, bool bwd, hipStream_t s);
+void launch_linrec_step(const LinrecArgs& a, bool is_bf16, hipStream_t s);
+
+// operators over rows of vocabulary logits [N, V] (unit stride along V, any row stride; bf16 or
+// fp32): topk.hip, distill.hip, filter.hip
+constexpr int kRowMaxV = 262144;  // distill.hip keeps one bit a token in LDS
+constexpr int kRowMaxK = 256;     // recorded teacher entries a row
+struct RowArgs {
+  const void* logits; long ld; int N, V; bool is_bf16;
+};
+// the k largest logits of each row (ties: the lowest index first) and log sum exp(logit * inv_t)
+void launch_topk(const RowArgs& r, int k, float inv_t, float* values, int* indices, float* lse,
+                 hipStream_t s);
+struct DistillArgs {
+  RowArgs r;
+  const float* values; const int* indices; int k;  // [N, k] recorded entries
+  const float* lse;            // optional [N]: the teacher's log-sum-exp (its rest mass counts)
+  const int* targets;          // optional [N]
+  float alpha, temperature, scale;
+  const float* gscale;         // optional device scalar that multiplies the gradient
+  float* row_loss;             // [N]
+  void* grad; long grad_ld; bool grad_bf16;  // optional [N, V]
+  float* loss;                 // optional: scale * sum of the row losses
+};
+void launch_distill(const DistillArgs& a, hipStream_t s);
+// one request setting: a per-row array, or a value for all rows
+struct PerRow { const float* p; float v; };
+struct FilterArgs {
+  RowArgs r;
+  const float* u;              // [N] uniform numbers
+  PerRow temperature, top_p, min_p;
+  const int* top_k; int top_k_all;
+  int* out;                    // [N] picked ids
+};
+void launch_filter_sample(const FilterArgs& a, hipStream_t s);
+
 }  // namespace dcr

@@ -2,8 +2,13 @@
 // torch.ops.load_library).  Only argument checking and stream plumbing lives here; every op
 // launches hand-written HIP kernels from the *.hip files on the current HIP stream.
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
+
+#include <algorithm>
+#include <cmath>
+#include <tuple>
 
 #include "kernels.h"
 #include "debug_env.h"
@@ -1940,6 +1945,287 @@ void prep(at::TensorList src, at::TensorList dst, at::IntArrayRef mode, at::Tens
   dcr::launch_prep(tab, cur_stream());
 }
 
+// ------------------------------------------------------------------------------------------
+// gated linear recurrence (linrec.hip) and operators over vocabulary rows (topk.hip, distill.hip,
+// filter.hip).  These take views: unit stride along the last dimension, any other strides.
+// ------------------------------------------------------------------------------------------
+// The tensors' device becomes the current one for the call, and the launch goes to its stream.
+struct OnDevice {
+  c10::DeviceGuard guard;
+  hipStream_t stream;
+  explicit OnDevice(const at::Tensor& t)
+      : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+};
+void check_on(const at::Tensor& t, const at::Tensor& like, at::ScalarType st, const char* name) {
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.scalar_type() == st, name, " must be ", st, ", got ", t.scalar_type());
+}
+void check_f32_or_bf16(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name,
+              " must be float32 or bfloat16, got ", t.scalar_type());
+}
+
+void check_seq3(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  check_on(t, like, like.scalar_type(), name);
+  TORCH_CHECK(t.sizes() == like.sizes(), name, " must be ", like.sizes(), ", got ", t.sizes());
+  TORCH_CHECK(t.size(2) == 1 || t.stride(2) == 1, name, " needs unit stride along its last dimension");
+}
+
+dcr::LinrecArgs linrec_args(const at::Tensor& x, const at::Tensor& f,
+                            const c10::optional<at::Tensor>& lengths,
+                            const c10::optional<at::Tensor>& starts, const char* op) {
+  check_f32_or_bf16(x, "x");
+  TORCH_CHECK(x.dim() == 3, op, ": x must be [T, B, H]");
+  check_seq3(x, x, "x");
+  check_seq3(f, x, "f");
+  TORCH_CHECK(x.size(0) < (1 << 30) && x.size(1) < (1 << 30) && x.size(2) < (1 << 30) &&
+                  x.size(1) * x.size(2) < (1LL << 31), op, ": sizes too large");
+  dcr::LinrecArgs a{};
+  a.T = (int)x.size(0); a.B = (int)x.size(1); a.H = (int)x.size(2);
+  a.x = x.data_ptr(); a.x_t = x.stride(0); a.x_b = x.stride(1);
+  a.f = f.data_ptr(); a.f_t = f.stride(0); a.f_b = f.stride(1);
+  if (has(lengths)) {
+    check_on(*lengths, x, at::kInt, "lengths");
+    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == a.B && lengths->is_contiguous(),
+                op, ": lengths must be [B], contiguous");
+    a.lengths = ptr<int>(*lengths);
+  }
+  if (has(starts)) {
+    check_on(*starts, x, at::kBool, "starts");
+    TORCH_CHECK(starts->dim() == 2 && starts->size(0) == a.T && starts->size(1) == a.B,
+                op, ": starts must be [T, B]");
+    a.starts = ptr<unsigned char>(*starts);
+    a.starts_t = starts->stride(0); a.starts_b = starts->stride(1);
+  }
+  return a;
+}
+const float* linrec_state(const c10::optional<at::Tensor>& t, const at::Tensor& x,
+                          const char* name) {
+  if (!has(t)) return nullptr;
+  check_on(*t, x, at::kFloat, name);
+  TORCH_CHECK(t->dim() == 2 && t->size(0) == x.size(1) && t->size(1) == x.size(2) &&
+                  t->is_contiguous(), name, " must be [B, H], contiguous");
+  return ptr<float>(*t);
+}
+// an output in the layout of `x` (a batch-first view stays one)
+at::Tensor linrec_out(const at::Tensor& x) {
+  at::Tensor t = at::empty_like(x);
+  return t.stride(-1) == 1 || t.size(-1) == 1 ? t : at::empty(x.sizes(), x.options());
+}
+at::Tensor linrec_pairs(dcr::LinrecArgs& a, const dcr::LinrecPlan& q, const at::TensorOptions& o) {
+  if (q.segs <= 1) return at::Tensor();
+  at::Tensor w = at::empty({2, q.segs, a.B, a.H}, o);
+  a.sumA = ptr<float>(w);
+  a.sumB = a.sumA + (size_t)q.segs * a.B * a.H;
+  return w;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linrec_fwd(
+    const at::Tensor& x, const at::Tensor& f, const c10::optional<at::Tensor>& h0,
+    const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& starts,
+    bool want_carry) {
+  dcr::LinrecArgs a = linrec_args(x, f, lengths, starts, "linrec_fwd");
+  a.h0 = linrec_state(h0, x, "h0");
+  OnDevice dev(x);
+  const auto o = x.options().dtype(at::kFloat);
+  at::Tensor h = linrec_out(x), hlast = at::empty({a.B, a.H}, o);
+  const dcr::LinrecPlan q = dcr::linrec_plan(a.T, a.B, a.H);
+  at::Tensor carry = at::empty({want_carry ? q.tiles : 0, a.B, a.H}, o);
+  if (a.T == 0 || x.numel() == 0) {
+    if (a.h0) hlast.copy_(*h0); else hlast.zero_();
+    return {h, hlast, carry};
+  }
+  a.h = h.data_ptr(); a.h_t = h.stride(0); a.h_b = h.stride(1);
+  a.hlast = ptr<float>(hlast);
+  a.carry = want_carry ? ptr<float>(carry) : nullptr;
+  const at::Tensor w = linrec_pairs(a, q, o);
+  dcr::launch_linrec(a, x.scalar_type() == at::kBFloat16, false, dev.stream);
+  return {h, hlast, carry};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linrec_bwd(
+    const at::Tensor& x, const at::Tensor& f, const at::Tensor& carry, const at::Tensor& dh,
+    const c10::optional<at::Tensor>& dlast, const c10::optional<at::Tensor>& lengths,
+    const c10::optional<at::Tensor>& starts) {
+  dcr::LinrecArgs a = linrec_args(x, f, lengths, starts, "linrec_bwd");
+  check_seq3(dh, x, "dh");
+  a.dlast = linrec_state(dlast, x, "dlast");
+  OnDevice dev(x);
+  const auto o = x.options().dtype(at::kFloat);
+  at::Tensor dx = linrec_out(x), df = linrec_out(f), dh0 = at::empty({a.B, a.H}, o);
+  const dcr::LinrecPlan q = dcr::linrec_plan(a.T, a.B, a.H);
+  check_on(carry, x, at::kFloat, "carry");
+  TORCH_CHECK(carry.dim() == 3 && carry.size(0) == q.tiles && carry.size(1) == a.B &&
+                  carry.size(2) == a.H && carry.is_contiguous(),
+              "linrec_bwd: carry must be the forward's, for the same sizes");
+  if (a.T == 0 || x.numel() == 0) {
+    if (a.dlast) dh0.copy_(*dlast); else dh0.zero_();
+    return {dx, df, dh0};
+  }
+  a.dh = dh.data_ptr(); a.dh_t = dh.stride(0); a.dh_b = dh.stride(1);
+  a.dx = dx.data_ptr(); a.dx_t = dx.stride(0); a.dx_b = dx.stride(1);
+  a.df = df.data_ptr(); a.df_t = df.stride(0); a.df_b = df.stride(1);
+  a.dh0 = ptr<float>(dh0);
+  a.carry = ptr<float>(carry);
+  const at::Tensor w = linrec_pairs(a, q, o);
+  dcr::launch_linrec(a, x.scalar_type() == at::kBFloat16, true, dev.stream);
+  return {dx, df, dh0};
+}
+
+at::Tensor linrec_step(const at::Tensor& x, const at::Tensor& f, at::Tensor& h,
+                       const c10::optional<at::Tensor>& starts) {
+  TORCH_CHECK(x.dim() == 2 && f.dim() == 2, "linrec_step: x and f must be [B, H]");
+  c10::optional<at::Tensor> st;
+  if (has(starts)) {
+    TORCH_CHECK(starts->dim() == 1, "linrec_step: starts must be [B]");
+    st = starts->unsqueeze(0);
+  }
+  dcr::LinrecArgs a = linrec_args(x.unsqueeze(0), f.unsqueeze(0), c10::nullopt, st, "linrec_step");
+  check_on(h, x, at::kFloat, "h");
+  TORCH_CHECK(h.sizes() == x.sizes() && h.is_contiguous(), "linrec_step: h must be [B, H], contiguous");
+  OnDevice dev(x);
+  at::Tensor y = linrec_out(x);
+  if (x.numel() == 0) return y;
+  a.h = y.data_ptr(); a.h_b = y.stride(0);
+  a.hlast = ptr<float>(h);
+  dcr::launch_linrec_step(a, x.scalar_type() == at::kBFloat16, dev.stream);
+  return y;
+}
+
+dcr::RowArgs row_args(const at::Tensor& logits, const char* op) {
+  check_f32_or_bf16(logits, "logits");
+  TORCH_CHECK(logits.dim() == 2, op, ": logits must be [N, V]");
+  const int64_t N = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V >= 1 && V <= dcr::kRowMaxV, op, ": vocabularies of 1 to ", dcr::kRowMaxV,
+              " entries, got ", V);
+  TORCH_CHECK(N < (1LL << 31), op, ": too many rows");
+  TORCH_CHECK(V == 1 || logits.stride(1) == 1, op, ": logits need unit stride along the vocabulary");
+  dcr::RowArgs r{};
+  r.logits = logits.data_ptr(); r.ld = logits.stride(0); r.N = (int)N; r.V = (int)V;
+  r.is_bf16 = logits.scalar_type() == at::kBFloat16;
+  return r;
+}
+void check_temperature(double t, const char* op) {
+  TORCH_CHECK(t > 0.0 && (float)t > 0.0f && std::isfinite((float)(1.0 / t)) && std::isfinite((float)t),
+              op, ": the temperature must be positive and finite, got ", t);
+}
+// [N] (or [N, k]) contiguous of one type
+void check_rows(const at::Tensor& t, const at::Tensor& logits, at::ScalarType st, int64_t k,
+                const char* name) {
+  check_on(t, logits, st, name);
+  const int64_t N = logits.size(0);
+  if (k < 0) {
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == N && t.is_contiguous(), name, " must be [N], contiguous");
+  } else {
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == N && t.size(1) == k && t.is_contiguous(), name,
+                " must be [N, ", k, "], contiguous");
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logits, int64_t k,
+                                                          double temperature) {
+  const dcr::RowArgs r = row_args(logits, "top_logits");
+  TORCH_CHECK(k >= 1 && k <= dcr::kRowMaxK && k <= r.V, "top_logits: k must be 1 to min(V, ",
+              dcr::kRowMaxK, "), got ", k);
+  check_temperature(temperature, "top_logits");
+  OnDevice dev(logits);
+  const auto o = logits.options().dtype(at::kFloat);
+  at::Tensor values = at::empty({r.N, k}, o), lse = at::empty({r.N}, o);
+  at::Tensor indices = at::empty({r.N, k}, o.dtype(at::kInt));
+  if (r.N > 0)
+    dcr::launch_topk(r, (int)k, (float)(1.0 / temperature), ptr<float>(values), ptr<int>(indices),
+                     ptr<float>(lse), dev.stream);
+  return {values, indices, lse};
+}
+
+void distill(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& indices,
+             const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& targets,
+             double alpha, double temperature, double scale,
+             const c10::optional<at::Tensor>& grad_scale, at::Tensor& row_loss,
+             const c10::optional<at::Tensor>& grad, const c10::optional<at::Tensor>& loss) {
+  dcr::DistillArgs a{};
+  a.r = row_args(logits, "distill");
+  TORCH_CHECK(values.dim() == 2, "distill: values must be [N, k]");
+  const int64_t k = values.size(1);
+  TORCH_CHECK(k >= 1 && k <= dcr::kRowMaxK, "distill: 1 to ", dcr::kRowMaxK,
+              " recorded entries a row, got ", k);
+  check_rows(values, logits, at::kFloat, k, "values");
+  check_rows(indices, logits, at::kInt, k, "indices");
+  check_rows(row_loss, logits, at::kFloat, -1, "row_loss");
+  check_temperature(temperature, "distill");
+  TORCH_CHECK(alpha >= 0.0 && alpha <= 1.0, "distill: alpha must be in [0, 1], got ", alpha);
+  TORCH_CHECK(alpha == 1.0 || has(targets), "distill: alpha < 1 needs targets");
+  TORCH_CHECK(std::isfinite(scale), "distill: scale must be finite");
+  a.values = ptr<float>(values); a.indices = ptr<int>(indices); a.k = (int)k;
+  if (has(lse)) { check_rows(*lse, logits, at::kFloat, -1, "lse"); a.lse = ptr<float>(*lse); }
+  if (has(targets)) {
+    check_rows(*targets, logits, at::kInt, -1, "targets");
+    a.targets = ptr<int>(*targets);
+  }
+  a.alpha = (float)alpha; a.temperature = (float)temperature; a.scale = (float)scale;
+  if (has(grad_scale)) {
+    check_on(*grad_scale, logits, at::kFloat, "grad_scale");
+    TORCH_CHECK(grad_scale->numel() == 1, "distill: grad_scale must be one number");
+    a.gscale = ptr<float>(*grad_scale);
+  }
+  a.row_loss = ptr<float>(row_loss);
+  if (has(grad)) {
+    check_f32_or_bf16(*grad, "grad");
+    TORCH_CHECK(grad->device() == logits.device() && grad->sizes() == logits.sizes() &&
+                    (a.r.V == 1 || grad->stride(1) == 1) && (a.r.N <= 1 || grad->stride(0) >= a.r.V),
+                "distill: grad must be [N, V] on the logits' device, unit stride along the "
+                "vocabulary, rows apart");
+    a.grad = grad->data_ptr(); a.grad_ld = grad->stride(0);
+    a.grad_bf16 = grad->scalar_type() == at::kBFloat16;
+  }
+  if (has(loss)) {
+    check_on(*loss, logits, at::kFloat, "loss");
+    TORCH_CHECK(loss->numel() == 1, "distill: loss must be one number");
+    a.loss = ptr<float>(*loss);
+  }
+  OnDevice dev(logits);
+  dcr::launch_distill(a, dev.stream);
+}
+
+at::Tensor filter_sample(const at::Tensor& logits, const at::Tensor& u, double temperature,
+                         int64_t top_k, double top_p, double min_p,
+                         const c10::optional<at::Tensor>& temperatures,
+                         const c10::optional<at::Tensor>& top_ks,
+                         const c10::optional<at::Tensor>& top_ps,
+                         const c10::optional<at::Tensor>& min_ps) {
+  dcr::FilterArgs a{};
+  a.r = row_args(logits, "filter_sample");
+  check_rows(u, logits, at::kFloat, -1, "u");
+  a.u = ptr<float>(u);
+  TORCH_CHECK(temperature >= 0.0 && std::isfinite(temperature),
+              "filter_sample: the temperature must be finite and not negative, got ", temperature);
+  TORCH_CHECK(top_k >= 0, "filter_sample: top_k must not be negative, got ", top_k);
+  TORCH_CHECK(top_p >= 0.0 && top_p <= 1.0, "filter_sample: top_p must be in [0, 1], got ", top_p);
+  TORCH_CHECK(min_p >= 0.0 && min_p <= 1.0, "filter_sample: min_p must be in [0, 1], got ", min_p);
+  auto per_row = [&](const c10::optional<at::Tensor>& t, double v, const char* name) {
+    dcr::PerRow p{nullptr, (float)v};
+    if (has(t)) {
+      check_rows(*t, logits, at::kFloat, -1, name);
+      p.p = ptr<float>(*t);
+    }
+    return p;
+  };
+  a.temperature = per_row(temperatures, temperature, "temperature");
+  a.top_p = per_row(top_ps, top_p, "top_p");
+  a.min_p = per_row(min_ps, min_p, "min_p");
+  a.top_k_all = (int)std::min<int64_t>(top_k, a.r.V);
+  if (has(top_ks)) {
+    check_rows(*top_ks, logits, at::kInt, -1, "top_k");
+    a.top_k = ptr<int>(*top_ks);
+  }
+  OnDevice dev(logits);
+  at::Tensor out = at::empty({a.r.N}, logits.options().dtype(at::kInt));
+  a.out = ptr<int>(out);
+  if (a.r.N > 0) dcr::launch_filter_sample(a, dev.stream);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(dcr, m) {
@@ -2160,6 +2446,18 @@ TORCH_LIBRARY(dcr, m) {
       "gru_persist_bwd(Tensor Wg, Tensor Wc, Tensor dtop, Tensor(a!) dz, Tensor gates, "
       "Tensor h32, Tensor(b!) cnt, Tensor(c!) err, int spin_limit, bool cnt_zeroed=False, "
       "Tensor(d!)? ring0=None, Tensor(e!)? ring1=None, Tensor(f!)? db_part=None) -> ()");
+  m.def("linrec_fwd(Tensor x, Tensor f, Tensor? h0, Tensor? lengths, Tensor? starts, "
+        "bool want_carry) -> (Tensor, Tensor, Tensor)");
+  m.def("linrec_bwd(Tensor x, Tensor f, Tensor carry, Tensor dh, Tensor? dlast, Tensor? lengths, "
+        "Tensor? starts) -> (Tensor, Tensor, Tensor)");
+  m.def("linrec_step(Tensor x, Tensor f, Tensor(a!) h, Tensor? starts) -> Tensor");
+  m.def("top_logits(Tensor logits, int k, float temperature) -> (Tensor, Tensor, Tensor)");
+  m.def("distill(Tensor logits, Tensor values, Tensor indices, Tensor? lse, Tensor? targets, "
+        "float alpha, float temperature, float scale, Tensor? grad_scale, Tensor(a!) row_loss, "
+        "Tensor(b!)? grad, Tensor(c!)? loss) -> ()");
+  m.def("filter_sample(Tensor logits, Tensor u, float temperature, int top_k, float top_p, "
+        "float min_p, Tensor? temperatures=None, Tensor? top_ks=None, Tensor? top_ps=None, "
+        "Tensor? min_ps=None) -> Tensor");
   m.def("segsum(Tensor X, Tensor? ids, int V, Tensor(a!) out, Tensor(b!) workspace, bool accumulate, "
         "Tensor? perm=None) -> ()");
   m.def("segsum_workspace(int N, int W, int V) -> int", [](int64_t N, int64_t W, int64_t V) -> int64_t {
@@ -2204,4 +2502,10 @@ TORCH_LIBRARY_IMPL(dcr, CUDA, m) {
   m.impl("embed_dropout", &embed_dropout);
   m.impl("sample_step", &sample_step);
   m.impl("gru_persist_bwd", &gru_persist_bwd);
+  m.impl("linrec_fwd", &linrec_fwd);
+  m.impl("linrec_bwd", &linrec_bwd);
+  m.impl("linrec_step", &linrec_step);
+  m.impl("top_logits", &top_logits);
+  m.impl("distill", &distill);
+  m.impl("filter_sample", &filter_sample);
 }

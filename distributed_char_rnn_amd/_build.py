@@ -70,6 +70,11 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wno-unused-r
           "-ffp-contract=fast"]
 # per-kernel register / scratch report of every device compile (parsed into _C.resources.json)
 DEV_FLAGS = ["-Rpass-analysis=kernel-resource-usage"]
+# No packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong
+# results on this hardware now and then.  (The host pass warns that it does not know the feature,
+# which is harmless.)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+NO_PACKED_F32_SOURCES = ("linrec.hip", "topk.hip", "distill.hip", "filter.hip")
 RESOURCES = os.path.join(PKG_DIR, "_C.resources.json")
 # Sources whose kernels spin on each other across workgroups (persistent hand-offs, in-launch
 # waits).  None of their kernels may spill to scratch: at the register limit this compiler has
@@ -115,7 +120,7 @@ def source_hash() -> str:
     import hashlib
 
     h = hashlib.sha256()
-    h.update(" ".join(COMMON + DEV_FLAGS).encode())
+    h.update(" ".join(COMMON + DEV_FLAGS + NO_PACKED_F32 + list(NO_PACKED_F32_SOURCES)).encode())
     for f in sorted(glob.glob(os.path.join(CSRC, "*"))):
         if os.path.isfile(f):
             h.update(os.path.basename(f).encode() + b"\0")
@@ -188,7 +193,8 @@ def _build_locked(force: bool, jobs: int | None, verbose: bool) -> str:
                                                               os.path.exists(res)):
             return obj, None
         if src.endswith(".hip"):
-            cmd = [hipcc, *COMMON, *DEV_FLAGS, "-I", CSRC, "-c", src, "-o", obj]
+            own = NO_PACKED_F32 if os.path.basename(src) in NO_PACKED_F32_SOURCES else []
+            cmd = [hipcc, *COMMON, *DEV_FLAGS, *own, "-I", CSRC, "-c", src, "-o", obj]
         else:  # torch bindings: host-only C++ (no device code), compiled by the host compiler
             cmd = [_cxx(), "-O2", "-std=c++17", "-fPIC", "-I", CSRC, *cflags, "-c", src, "-o", obj]
         if verbose:
