@@ -20,116 +20,140 @@ namespace dcr {
 
 template <typename T, typename G, int NT, int EPT>
 __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
+  constexpr int kE = NT < kRowMaxK ? kRowMaxK / NT : 1;  // entries a thread
+  constexpr bool kKeep = EPT > 0 && EPT <= 32;  // room for the exponentials beside the row
+  constexpr int kKept = kKeep ? EPT / 4 : 1;
   extern __shared__ unsigned bits[];
-  __shared__ float red[NT / 64];
-  __shared__ float et[kRowMaxK], ez[kRowMaxK];  // entries: t / T, the student's z
-  __shared__ int ei[kRowMaxK];                  // column; -1: no entry
-  __shared__ unsigned char first[kRowMaxK];     // the first entry of its column
-  __shared__ int twice;
+  __shared__ float red[(3 + 5 + 2) * (NT / 64)];
+  __shared__ int ei[kRowMaxK], twice;
+  __shared__ float eq[kRowMaxK];  // q of the entries, for columns recorded twice
   const long n = blockIdx.x;
   const int tid = threadIdx.x, V = a.r.V, k = a.k;
   const T* z = reinterpret_cast<const T*>(a.r.logits) + n * a.r.ld;
   G* grad = a.grad ? reinterpret_cast<G*>(a.grad) + n * a.grad_ld : nullptr;
-  const float inv_t = 1.0f / a.temperature;
-  const int y = a.targets ? a.targets[n] : 0;
+  const float inv_t = 1.0f / a.temperature, c_t = inv_t * 1.44269504088896341f;
+  constexpr float c_1 = 1.44269504088896341f;
+  const int y = a.targets ? a.targets[n] : -1;
   const bool skip = a.targets && (y < 0 || y >= V);
   const bool ce = a.targets && a.alpha < 1.0f;
   const bool two = ce && inv_t != 1.0f;  // a second exponential an element
 
+  // ---- the entries: column (-1: none), t / T, the student's z
+  int i_e[kE];
+  float t_e[kE], z_e[kE];
+  bool first[kE];  // the first entry of its column
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    const int j = e * NT + tid;
+    i_e[e] = j < k ? a.indices[n * k + j] : -1;
+    if (i_e[e] >= V) i_e[e] = -1;
+    t_e[e] = i_e[e] >= 0 ? a.values[n * k + j] * inv_t : -INFINITY;
+  }
+  const float z_y = ce && !skip ? (float)z[y] : 0.f;
+  Row<T, NT, EPT> row(z, V);
   for (int i = tid; i < (V + 31) / 32; i += NT) bits[i] = 0;
   if (tid == 0) twice = 0;
   __syncthreads();
-  for (int j = tid; j < k; j += NT) {
-    const int i = a.indices[n * k + j];
-    const bool ok = i >= 0 && i < V;
-    ei[j] = ok ? i : -1;
-    et[j] = ok ? a.values[n * k + j] * inv_t : -INFINITY;
-    ez[j] = ok ? (float)z[i] : -INFINITY;
-    first[j] = ok;
-    if (ok && (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1)) twice = 1;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    const int i = i_e[e];
+    first[e] = i >= 0;
+    z_e[e] = i >= 0 ? (float)z[i] : -INFINITY;
+    if (i >= 0 && (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1)) twice = 1;
+    if (e * NT + tid < k) ei[e * NT + tid] = i;
   }
-  Row<T, NT, EPT> row(z, V);
   __syncthreads();
   if (twice) {  // a column recorded more than once: its first entry stands for it
-    for (int j = tid; j < k; j += NT)
-      for (int i = 0; i < j; ++i)
-        if (ei[i] == ei[j]) first[j] = 0;
-    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kE; ++e)
+      for (int j = 0; j < e * NT + tid && first[e]; ++j)
+        if (ei[j] == i_e[e]) first[e] = false;
   }
   // the entries' nibble of four columns
   auto marked = [&](int col) -> unsigned {
-    return col < V ? bits[col >> 5] >> (col & 31) & 15u : 15u;
+    return col < V ? bits[col >> 5] >> (col & 31) & 15u : 0u;
   };
-
-  // ---- the rest: maximum, then the sums at T and at 1
-  float mr = -INFINITY;
-  row.visit([&](int col, float (&x)[4], int) {
-    const unsigned q = marked(col);
+  auto rest_of = [&](float (&x)[4], int col) {  // a row that is read again loses them each time
+    if constexpr (EPT == 0) {
+      const unsigned q = marked(col);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (!(q >> j & 1)) mr = fmaxf(mr, x[j]);
-  });
-  mr = block_reduce<NT>(mr, red, MaxOp());
-  float sr = 0.f, sr1 = 0.f;
-  row.visit([&](int col, float (&x)[4], int) {
-    const unsigned q = marked(col);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (!(q >> j & 1) && x[j] != -INFINITY) {
-        sr += __expf((x[j] - mr) * inv_t);
-        if (two) sr1 += __expf(x[j] - mr);
-      }
-  });
-  sr = block_reduce<NT>(sr, red, AddOp());
-  sr1 = two ? block_reduce<NT>(sr1, red, AddOp()) : sr;
-
-  // ---- the entries
-  float mk = -INFINITY, mt = -INFINITY;
-  for (int j = tid; j < k; j += NT) {
-    mk = fmaxf(mk, ez[j]);
-    mt = fmaxf(mt, et[j]);
-  }
-  mk = block_reduce<NT>(mk, red, MaxOp());
-  mt = block_reduce<NT>(mt, red, MaxOp());
-  const float m = fmaxf(mr, mk);
-  float sk = 0.f, sk1 = 0.f, st = 0.f;
-  for (int j = tid; j < k; j += NT) {
-    if (first[j] && ez[j] != -INFINITY) {
-      sk += __expf((ez[j] - mk) * inv_t);
-      if (two) sk1 += __expf(ez[j] - mk);
+      for (int j = 0; j < 4; ++j)
+        if (q >> j & 1) x[j] = -INFINITY;
     }
-    if (et[j] != -INFINITY) st += __expf(et[j] - mt);
+  };
+  if constexpr (EPT > 0) row.erase(marked);
+
+  // ---- maxima: of the rest, of the entries' z and t
+  float top[3] = {-INFINITY, -INFINITY, -INFINITY};
+  row.visit([&](int col, float (&x)[4], int) {
+    rest_of(x, col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[0] = fmaxf(top[0], x[j]);
+  });
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    top[1] = fmaxf(top[1], z_e[e]);
+    top[2] = fmaxf(top[2], t_e[e]);
   }
-  sk = block_reduce<NT>(sk, red, AddOp());
-  sk1 = two ? block_reduce<NT>(sk1, red, AddOp()) : sk;
-  st = block_reduce<NT>(st, red, AddOp());
+  block_reduce_each<NT, 3>(top, red, MaxOp());
+  const float mr = top[0], mk = top[1], mt = top[2], m = fmaxf(mr, mk);
+  const float mr0 = mr == -INFINITY ? 0.f : mr;  // (an empty rest sums to 0)
+
+  // ---- sums at T and at 1: of the rest, of the entries' z; and of the entries' t
+  float sum[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  float et[kKept][4], e1[kKept][4];
+  row.visit([&](int col, float (&x)[4], int c) {
+    rest_of(x, col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = x[j] - mr0, p = __builtin_amdgcn_exp2f(d * c_t);
+      sum[0] += p;
+      if (kKeep) et[kKeep ? c : 0][j] = p;
+      if (two) {
+        const float p1 = __builtin_amdgcn_exp2f(d * c_1);
+        sum[1] += p1;
+        if (kKeep) e1[kKeep ? c : 0][j] = p1;
+      }
+    }
+  });
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    if (first[e] && z_e[e] != -INFINITY) {
+      sum[2] += __expf((z_e[e] - mk) * inv_t);
+      if (two) sum[3] += __expf(z_e[e] - mk);
+    }
+    if (t_e[e] != -INFINITY) sum[4] += __expf(t_e[e] - mt);
+  }
+  block_reduce_each<NT, 5>(sum, red + 3 * (NT / 64), AddOp());
+  const float sr = sum[0], sr1 = two ? sum[1] : sum[0];
+  const float sk = sum[2], sk1 = two ? sum[3] : sum[2];
 
   // a skipped row, and one whose mask leaves no column, has neither loss nor gradient
   const bool none = skip || (m == -INFINITY && sr == 0.f && sk == 0.f);
-  const float wr = mr == -INFINITY ? 0.f : __expf((mr - m) * inv_t);
-  const float wk = mk == -INFINITY ? 0.f : __expf((mk - m) * inv_t);
-  const float lse = m * inv_t + __logf(sr * wr + sk * wk);
-  const float wr1 = mr == -INFINITY ? 0.f : __expf(mr - m);
-  const float wk1 = mk == -INFINITY ? 0.f : __expf(mk - m);
-  const float lse1 = m + __logf(sr1 * wr1 + sk1 * wk1);
+  // log-sum-exps over m: no logit is scaled by itself, so the lowest values of the type stay finite
+  const float dr = mr == -INFINITY ? -INFINITY : mr - m, dk = mk == -INFINITY ? -INFINITY : mk - m;
+  const float lse = __logf(sr * __expf(dr * inv_t) + sk * __expf(dk * inv_t));
+  const float lse1 = __logf(sr1 * __expf(dr) + sk1 * __expf(dk));
   const bool told = a.lse != nullptr;
   // entries that hold nothing say nothing
   const float alpha = !told && mt == -INFINITY ? 0.f : a.alpha;
-  const float lt = told ? a.lse[n] : mt + __logf(st);
-  float sq = 0.f, kl = 0.f;
-  for (int j = tid; j < k; j += NT)
-    if (et[j] != -INFINITY) {
-      const float lq = et[j] - lt, q = __expf(lq);
-      sq += q;
-      if (q > 0.f) kl += q * (lq - (ez[j] * inv_t - lse));
-    }
-  sq = block_reduce<NT>(sq, red, AddOp());
-  kl = block_reduce<NT>(kl, red, AddOp());
-  float rest = told ? fmaxf(0.f, 1.0f - sq) : 0.f;
+  const float lt = told ? a.lse[n] : mt + __logf(sum[4]);
+  float q_e[kE], say[2] = {0.f, 0.f};  // sum of q, divergence at the entries
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    const float lq = t_e[e] - lt;
+    q_e[e] = t_e[e] != -INFINITY ? __expf(lq) : 0.f;
+    say[0] += q_e[e];
+    if (t_e[e] != -INFINITY && !(q_e[e] <= 0.f)) say[1] += q_e[e] * (lq - ((z_e[e] - m) * inv_t - lse));
+    if (e * NT + tid < k) eq[e * NT + tid] = q_e[e];
+  }
+  block_reduce_each<NT, 2>(say, red + 8 * (NT / 64), AddOp());
+  if (NT == 64) __syncthreads();  // eq
+  float rest = told ? fmaxf(0.f, 1.0f - say[0]) : 0.f, kl = say[1];
   if (mr == -INFINITY) rest = 0.f;  // no column to hold it
-  if (rest > 0.f) kl += rest * (__logf(rest) - (mr * inv_t + __logf(sr) - lse));
+  if (rest > 0.f) kl += rest * (__logf(rest) - (dr * inv_t + __logf(sr) - lse));
   float loss = alpha != 0.f ? alpha * a.temperature * a.temperature * kl : 0.f;
-  if (ce) loss += (1.0f - a.alpha) * (lse1 - (float)z[skip ? 0 : y]);
+  if (ce) loss += (1.0f - a.alpha) * (lse1 - (z_y - m));
   if (tid == 0) a.row_loss[n] = none ? 0.f : loss;
   if (!grad) return;
 
@@ -137,22 +161,35 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   const float scale = a.scale * (a.gscale ? *a.gscale : 1.0f);
   const float ct = alpha * a.temperature * scale, c1 = ce ? (1.0f - a.alpha) * scale : 0.f;
   // weights of exp((z - mr) / T) and exp(z - mr) off the entries
-  const float ft = mr == -INFINITY ? 0.f
-                                   : ct * (__expf(mr * inv_t - lse) - (rest > 0.f ? rest / sr : 0.f));
-  const float f1 = mr == -INFINITY ? 0.f : c1 * __expf(mr - lse1);
-  row.visit([&](int col, float (&x)[4], int) {
+  float ft = ct * (__expf(dr * inv_t - lse) - (rest > 0.f ? rest / sr : 0.f));
+  float f1 = c1 * __expf(dr - lse1);
+  if (mr == -INFINITY) ft = f1 = 0.f;
+  if (!two) ft += f1, f1 = 0.f;
+  if (none) ft = f1 = 0.f;
+  // the target's chunk, for the thread that holds it
+  const int cy = ce && !none && (y >> 2) % NT == tid ? (y >> 2) / NT : -1;
+  row.visit([&](int col, float (&x)[4], int c) {
     const unsigned q = marked(col);
+    rest_of(x, col);
     float g[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float e = 0.f;
-      if (x[j] != -INFINITY) {
-        const float et_ = __expf((x[j] - mr) * inv_t);
-        e = ft * et_ + f1 * (two ? __expf(x[j] - mr) : et_);
+      if (kKeep) {
+        g[j] = ft * et[kKeep ? c : 0][j];
+        if (two) g[j] += f1 * e1[kKeep ? c : 0][j];
+      } else {
+        const float d = x[j] - mr0;
+        g[j] = ft * __builtin_amdgcn_exp2f(d * c_t);
+        if (two) g[j] += f1 * __builtin_amdgcn_exp2f(d * c_1);
       }
-      if (ce && col + j == y) e -= c1;
-      g[j] = none ? 0.f : e;
     }
+    if (c == cy)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((y & 3) == j) g[j] -= c1;
+    if (none)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = 0.f;
     if (q == 0 && col + 3 < V) {
       typename Vec4<G>::type o;
 #pragma unroll
@@ -164,15 +201,16 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
         if (!(q >> j & 1) && col + j < V) grad[col + j] = (G)g[j];
     }
   });
-  for (int j = tid; j < k; j += NT) {
-    if (!first[j]) continue;
-    float q = et[j] != -INFINITY ? __expf(et[j] - lt) : 0.f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    if (!first[e]) continue;
+    float q = q_e[e];
     if (twice)
-      for (int i = j + 1; i < k; ++i)
-        if (ei[i] == ei[j] && et[i] != -INFINITY) q += __expf(et[i] - lt);
-    float e = ct != 0.f ? ct * (__expf(ez[j] * inv_t - lse) - q) : 0.f;
-    if (ce) e += c1 * __expf(ez[j] - lse1) - (ei[j] == y ? c1 : 0.f);
-    grad[ei[j]] = (G)(none ? 0.f : e);
+      for (int j = e * NT + tid + 1; j < k; ++j)
+        if (ei[j] == i_e[e]) q += eq[j];
+    float g = ct != 0.f ? ct * (__expf((z_e[e] - m) * inv_t - lse) - q) : 0.f;
+    if (ce) g += c1 * __expf(z_e[e] - m - lse1) - (i_e[e] == y ? c1 : 0.f);
+    grad[i_e[e]] = (G)(none ? 0.f : g);
   }
 }
 

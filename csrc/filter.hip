@@ -10,6 +10,16 @@
 // The answer is a whole number that a value next to a border decides, so weights are computed in
 // 64 bits and added as whole numbers of 2^-44: sums are exact in any order, and a border is off
 // by some 2^-44 of the largest weight a token.  2^44 times 262144 tokens fits 63 bits.
+//
+// One workgroup a row, the row in registers: it is read once.  Three ways to the kept set:
+//   top_k <= 256      the first top_k meet in LDS and are ordered there (as in topk.hip); only
+//                     they are weighed.
+//   top_p, large top_k  counts and weights by value interval (kBins of them, in LDS) find the
+//                     interval that holds a border; its entries meet in LDS, are ordered, and the
+//                     border is the one entry in front of which less than the target lies.
+//   otherwise         nothing to find: min_p is a bound on the value.
+// An interval that holds more than kList entries (rows of many equal values) is halved by values
+// until one value is left, as a whole: slow, and hardly ever.
 #include "vocab_row.h"
 
 namespace dcr {
@@ -17,44 +27,127 @@ namespace dcr {
 namespace {
 
 typedef unsigned long long u64;
-constexpr double kOne = 17592186044416.0;  // 2^44
+constexpr int kList = 1024;
 
-__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 __device__ __forceinline__ float of_row(const PerRow& p, long n) { return p.p ? p.p[n] : p.v; }
 
+// 2^44 exp((x - m) / temperature), as a number and rounded.  2^f on [-1/2, 1/2] by its power
+// series to f^11 (the rest is below 2^-47); adding 2^52 leaves the rounded number in the low bits.
 struct Weigh {
   float m;
-  double inv_t;
+  double c;  // log2(e) / temperature
   __device__ __forceinline__ double real(float x) const {
-    if (x == m) return 1.0;
-    return x == -INFINITY || m == INFINITY ? 0.0 : exp(((double)x - (double)m) * inv_t);
+    if (x == m) return 17592186044416.0;
+    if (x == -INFINITY || m == INFINITY) return 0.0;
+    const double y = fmax(((double)x - (double)m) * c, -64.0);
+    const double n = rint(y), f = y - n;
+    double p = 4.4455382718708114e-10;  // ln(2)^k / k!, k = 11 .. 0
+    p = fma(p, f, 7.0549116208011234e-09);
+    p = fma(p, f, 1.0178086009239699e-07);
+    p = fma(p, f, 1.3215486790144307e-06);
+    p = fma(p, f, 1.5252733804059841e-05);
+    p = fma(p, f, 1.5403530393381608e-04);
+    p = fma(p, f, 1.3333558146428443e-03);
+    p = fma(p, f, 9.6181291076284772e-03);
+    p = fma(p, f, 5.5504108664821580e-02);
+    p = fma(p, f, 2.4022650695910071e-01);
+    p = fma(p, f, 6.9314718055994531e-01);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)n + 44);
   }
-  __device__ __forceinline__ u64 operator()(float x) const { return (u64)(real(x) * kOne + 0.5); }
+  __device__ __forceinline__ u64 whole(double w) const {
+    return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 operator()(float x) const { return whole(real(x)); }
 };
+
+template <int NT>
+struct Work {  // LDS of one workgroup
+  static constexpr int kBins = NT == 64 ? 256 : 1024;
+  static constexpr int kCap = NT == 64 ? 256 : kList;
+  float redf[NT / 64];
+  int redi[NT / 64];
+  u64 redu[NT / 64];
+  float lv[kCap];
+  int li[kCap];
+  u64 lw[kCap];
+  union {
+    struct { u64 mass[kBins]; int count[kBins]; } bin;
+    struct { float v[kRowMaxK]; int i[kRowMaxK]; u64 w[kRowMaxK]; } top;  // ordered entries
+    float gm[NT == 64 ? 1 : kGroups];
+  };
+  int n, chosen, chosen_last;
+  float reached, chosen_value;
+  u64 chosen_mass, chosen_total;
+  int bin_at, bin_count;
+  u64 bin_mass;
+};
+
+// The bin in which the running number (of entries, or of weight) from bin 0 on reaches `target`:
+// s.bin_at, and what lies in front of it in s.bin_count / s.bin_mass.  s.bin_at is kBins if it is
+// never reached.
+template <int NT, bool BY_MASS>
+__device__ __forceinline__ void find_bin(Work<NT>& s, u64 target) {
+  constexpr int kPer = Work<NT>::kBins / 64;
+  if (threadIdx.x == 0) s.bin_at = Work<NT>::kBins;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int b0 = threadIdx.x * kPer;
+    int c = 0;
+    u64 w = 0;
+    for (int i = 0; i < kPer; ++i) c += s.bin.count[b0 + i], w += s.bin.mass[b0 + i];
+    int cb = wave_scan(c) - c;
+    u64 wb = wave_scan(w) - w;
+    const u64 from = BY_MASS ? wb : (u64)cb, to = from + (BY_MASS ? w : (u64)c);
+    if (from < target && target <= to) {
+      int i = b0;
+      for (; i < b0 + kPer - 1; ++i) {
+        const u64 next = BY_MASS ? wb + s.bin.mass[i] : (u64)(cb + s.bin.count[i]);
+        if (next >= target) break;
+        cb += s.bin.count[i];
+        wb += s.bin.mass[i];
+      }
+      s.bin_at = i;
+      s.bin_count = cb;
+      s.bin_mass = wb;
+    }
+  }
+  __syncthreads();
+}
+
+// chunks of four a thread that a row in LDS may take: 32 KB for 256 threads, 128 KB for 1024
+template <typename T, int NT>
+constexpr int lds_chunks() { return (NT == 256 ? 32768 : 131072) / (NT * 4 * (int)sizeof(T)); }
 
 }  // namespace
 
+// EPT: elements a thread in registers; 0: the row is read again by every visit; -1: it is in LDS
 template <typename T, int NT, int EPT>
 __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
-  constexpr int NW = NT / 64;
-  constexpr int kMaxChunks = EPT ? EPT / 4 : kRowMaxV / (NT * 4);
-  __shared__ float redf[NW];
-  __shared__ int redi[NW];
-  __shared__ u64 redu[NW];
+  constexpr int NW = NT / 64, kBins = Work<NT>::kBins, kCap = Work<NT>::kCap;
+  constexpr int kMaxChunks = EPT > 0 ? EPT / 4 : EPT < 0 ? lds_chunks<T, NT>() : kRowMaxV / (NT * 4);
+  extern __shared__ char held[];
+  __shared__ Work<NT> s;
   __shared__ u64 part[kMaxChunks * NW];
-  __shared__ int found;
-  __shared__ u64 left;
   const long n = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, V = a.r.V;
-  Row<T, NT, EPT> row(reinterpret_cast<const T*>(a.r.logits) + n * a.r.ld, V);
+  const T* logits = reinterpret_cast<const T*>(a.r.logits) + n * a.r.ld;
+  auto row = [&] {
+    if constexpr (EPT < 0) return RowLds<T, NT>(logits, V, held);
+    else return Row<T, NT, EPT>(logits, V);
+  }();
 
-  float m = -INFINITY;
+  float m = -INFINITY, low = INFINITY;
   row.visit([&](int, float (&x)[4], int) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, x[j]);
+    for (int j = 0; j < 4; ++j) {
+      m = fmaxf(m, x[j]);
+      if (x[j] > -INFINITY) low = fminf(low, x[j]);
+    }
   });
-  m = block_reduce<NT>(m, redf, MaxOp());
-  const float temp = of_row(a.temperature, n);
+  if (tid == 0) s.n = 0;
+  m = block_reduce<NT>(m, s.redf, MaxOp());
+  const float temp = uniform(of_row(a.temperature, n));
   if (!(temp > 0.f) || m == -INFINITY) {  // the first of the order
     int at = V;
     row.visit([&](int col, float (&x)[4], int) {
@@ -62,153 +155,276 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       for (int j = 0; j < 4; ++j)
         if (clean(x[j]) == m) at = min(at, col + j);
     });
-    at = block_reduce<NT>(at, redi, MinOp());
+    at = block_reduce<NT>(at, s.redi, MinOp());
     if (tid == 0) a.out[n] = at;
     return;
   }
-  const Weigh weigh{m, 1.0 / (double)temp};
-  const float top_p = of_row(a.top_p, n), min_p = of_row(a.min_p, n);
-  const int want = a.top_k ? a.top_k[n] : a.top_k_all;
+  low = block_reduce<NT>(low, s.redf, MinOp());
+  const Weigh weigh{m, 1.4426950408889634 / (double)temp};
+  const float top_p = uniform(of_row(a.top_p, n)), min_p = of_row(a.min_p, n);
+  const int want = uniform(a.top_k ? a.top_k[n] : a.top_k_all);
+  // (a NaN min_p: no floor)
+  const double floor_w = (min_p > 1.0f ? 1.0 : (double)min_p) * 17592186044416.0;
+  double u = (double)a.u[n];
+  if (!(u > 0.0)) u = 0.0;
+  auto place = [&](u64 total) {  // u of the whole; total is at least the first's 2^44
+    const double at = u * (double)total;
+    const u64 r = at < (double)total ? (u64)at : total - 1;
+    return r < total ? r : total - 1;
+  };
+  // the least whole number that is not below p of the total (at least 1: the first is kept)
+  auto share = [&](u64 total) {
+    const double t = ceil((double)top_p * (double)total);
+    return t >= 1.0 ? (u64)t : (u64)1;
+  };
+
+  if (want > 0 && want <= kRowMaxK && want < V) {
+    // ---- the first `want`, ordered in LDS
+    int c = 0;
+    if constexpr (NT != 64) {
+      const float f = reached_by<NT>(row, s.gm, &s.reached, want);
+      // (entries of -inf weigh nothing: fewer than `want` others are all that is needed)
+      collect<NT>(row, s.lv, s.li, &s.n, kCap, [&](float x, int) {
+        return x >= f && x > -INFINITY;
+      });
+      c = uniform(s.n);
+    }
+    if (NT == 64 || c > kCap) {
+      const Cut cut = cut_by_count<NT>(row, s.redi, m, low, want);
+      if (tid == 0) s.n = 0;
+      __syncthreads();
+      collect<NT>(row, s.lv, s.li, &s.n, kCap, [&](float x, int col) {
+        return x > -INFINITY && (x > cut.value || (x == cut.value && col <= cut.last));
+      });
+      c = uniform(s.n);
+    }
+    for (int i = tid; i < c; i += NT) {
+      const float y = s.lv[i];
+      const int col = s.li[i];
+      int at = 0;
+      for (int j = 0; j < c; ++j) at += s.lv[j] > y || (s.lv[j] == y && s.li[j] < col);
+      if (at < want) {
+        s.top.v[at] = y;
+        s.top.i[at] = col;
+        s.top.w[at] = weigh(y);
+      }
+    }
+    c = min(c, want);
+    __syncthreads();
+    if (w == 0) {
+      constexpr int kPer = kRowMaxK / 64;
+      u64 q[kPer], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = lane * kPer + i;
+        q[i] = at < c ? s.top.w[at] : 0;
+        sum += q[i];
+      }
+      u64 before = wave_scan(sum) - sum;
+      const u64 total = lane_value(before + sum, 63);
+      const u64 target = top_p < 1.0f ? share(total) : ~0ull;
+      int kept = 0;
+      u64 mass = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int at = lane * kPer + i;
+        const bool in = at < c && before < target &&
+                        (at == 0 || !(weigh.real(s.top.v[at]) < floor_w));
+        before += q[i];
+        if (in) kept = at + 1, mass += q[i];
+      }
+      kept = wave_reduce(kept, MaxOp());
+      mass = wave_reduce(mass, AddOp());
+      if (lane == 0) s.chosen = kept, s.chosen_total = mass;
+    }
+    __syncthreads();
+    c = uniform(s.chosen);
+    const u64 r = place(s.chosen_total);
+    for (int i = tid; i < c; i += NT) {  // running weights in the order of the indices
+      const int col = s.top.i[i];
+      const u64 mine = s.top.w[i];
+      u64 before = 0;
+      for (int j = 0; j < c; ++j)
+        if (s.top.i[j] < col) before += s.top.w[j];
+      if (r >= before && r < before + mine) a.out[n] = col;
+    }
+    return;
+  }
 
   // kept so far: values above `cut`, and those equal to it up to column `last`
   float cut = -INFINITY;
   int last = V - 1;
   auto kept = [&](float x, int col) { return x > cut || (x == cut && col <= last); };
-  // the column of the need-th kept value equal to f
-  auto nth_equal = [&](float f, long need) {
-    int lo = -1, hi = last;
-    while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      int c = 0;
+  const bool by_k = want > 0 && want < V, by_p = top_p < 1.0f;
+  if (by_k || by_p) {
+    // ---- counts and weights of kBins intervals of x = (m - l) / temperature; from 32 on the
+    // weight rounds to 0, so where the intervals end there, what the last one drops is never drawn
+    const float inv_t = 1.0f / temp;
+    const float span = fminf((m - low) * inv_t, 32.0f);
+    const float per = span > 0.f ? (float)kBins / span : 0.f;
+    const bool clipped = !((m - low) * inv_t < 32.0f);
+    auto bin_of = [&](float x) {
+      const float d = (m - x) * inv_t * per;  // falls with x, also as rounded
+      return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+    };
+    for (int i = tid; i < kBins; i += NT) s.bin.count[i] = 0, s.bin.mass[i] = 0;
+    __syncthreads();
+    row.visit([&](int, float (&x)[4], int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x[j] > -INFINITY) {
+          const int b = x[j] == m ? 0 : bin_of(x[j]);
+          const u64 q = weigh(x[j]);
+          if (by_k) atomicAdd(&s.bin.count[b], 1);
+          if (q) atomicAdd(&s.bin.mass[b], q);
+        }
+    });
+    __syncthreads();
+    // the entry of a bin in front of which (with what lies in front of the bin) less than
+    // `target` entries or weight lies, and with which it does not: the last one kept
+    auto border = [&](int b, u64 in_front, u64 target, bool by_mass) {
+      if (tid == 0) s.n = 0;
+      __syncthreads();
+      collect<NT>(row, s.lv, s.li, &s.n, kCap, [&](float x, int col) {
+        return x > -INFINITY && (x == m ? 0 : bin_of(x)) == b && kept(x, col);
+      });
+      const int c = uniform(s.n);
+      if (c <= kCap) {
+        for (int i = tid; i < c; i += NT) s.lw[i] = weigh(s.lv[i]);
+        __syncthreads();
+        for (int i = tid; i < c; i += NT) {
+          const float y = s.lv[i];
+          const int col = s.li[i];
+          u64 count = 0, mass = 0;
+          for (int j = 0; j < c; ++j)
+            if (s.lv[j] > y || (s.lv[j] == y && s.li[j] < col)) ++count, mass += s.lw[j];
+          const u64 before = in_front + (by_mass ? mass : count);
+          if (before < target && target <= before + (by_mass ? s.lw[i] : 1)) {
+            s.chosen_value = y;
+            s.chosen_last = col;
+            s.chosen_mass = mass + s.lw[i];
+          }
+        }
+        __syncthreads();
+        cut = uniform(s.chosen_value);
+        last = uniform(s.chosen_last);
+        __syncthreads();
+        return uniform(s.chosen_mass);
+      }
+      // many entries: halve the bin's range of values
+      auto amount = [&](float f) {
+        u64 q = 0;
+        row.visit([&](int col, float (&x)[4], int) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (x[j] >= f && x[j] > -INFINITY && (x[j] == m ? 0 : bin_of(x[j])) == b &&
+                kept(x[j], col + j))
+              q += by_mass ? weigh(x[j]) : 1;
+        });
+        return block_reduce<NT>(q, s.redu, AddOp());
+      };
+      unsigned lo = key_of(low), hi = key_of(m) + 1;
+      u64 above = 0;  // amount(>= hi) in front of the target, which amount(>= lo) reaches
+      for (int round = 0; hi - lo > 1; ++round) {
+        const unsigned mid = split_key(lo, hi, round);
+        const u64 q = amount(float_of(mid));
+        if (in_front + q >= target) lo = mid; else hi = mid, above = q;
+      }
+      const float f = float_of(lo);
+      const u64 each = by_mass ? weigh(f) : 1;
+      const u64 need = (target - in_front - above + each - 1) / each;  // entries equal to f
+      int c0 = -1, c1 = V - 1;
+      while (c1 - c0 > 1) {
+        const int mid = c0 + (c1 - c0) / 2;
+        const int q = count_if<NT>(row, s.redi, [&](float x, int col) {
+          return x == f && col <= mid && kept(x, col);
+        });
+        if ((u64)q >= need) c1 = mid; else c0 = mid;
+      }
+      u64 mass = 0;
       row.visit([&](int col, float (&x)[4], int) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c += clean(x[j]) == f && col + j <= mid;
+        for (int j = 0; j < 4; ++j)
+          if (x[j] > -INFINITY && (x[j] == m ? 0 : bin_of(x[j])) == b && kept(x[j], col + j) &&
+              (x[j] > f || (x[j] == f && col + j <= c1)))
+            mass += weigh(x[j]);
       });
-      c = block_reduce<NT>(c, redi, AddOp());
-      if (c >= need) hi = mid; else lo = mid;
-    }
-    return hi;
-  };
-
-  if (want > 0 && want < V) {
-    unsigned lo = key_of(-INFINITY), hi = key_of(m) + 1;
-    int above = 0, have = V;
-    while (hi - lo > 1 && have != want) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      const float f = float_of(mid);
-      int c = 0;
-      row.visit([&](int, float (&x)[4], int) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c += x[j] >= f;
-      });
-      c = block_reduce<NT>(c, redi, AddOp());
-      if (c >= want) lo = mid, have = c; else hi = mid, above = c;
-    }
-    const float f = float_of(lo);
-    if (have != want) last = nth_equal(f, want - above);
-    cut = f;
-  }
-  auto mass = [&](auto&& pred) {
-    u64 s = 0;
-    row.visit([&](int col, float (&x)[4], int) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float y = clean(x[j]);
-        if (kept(y, col + j) && pred(y)) s += weigh(y);
+      mass = block_reduce<NT>(mass, s.redu, AddOp());
+      cut = f;
+      last = c1;
+      return mass;
+    };
+    u64 total = 0;  // the weight of the first top_k
+    bool all = !by_k;
+    if (by_k) {
+      find_bin<NT, false>(s, (u64)want);
+      const int b = uniform(s.bin_at);
+      // (fewer than top_k above -inf, or the rest weighs nothing: all weight is kept)
+      all = b == kBins || (clipped && b == kBins - 1);
+      if (!all) {
+        const u64 front = uniform(s.bin_mass);
+        total = front + border(b, (u64)uniform(s.bin_count), (u64)want, false);
       }
-    });
-    return block_reduce<NT>(s, redu, AddOp());
-  };
-  if (top_p < 1.0f) {
-    const double target = (double)top_p * (double)mass([](float) { return true; });
-    // mass(>= lo) >= target > mass(>= hi)
-    unsigned lo = max(key_of(cut), key_of(-INFINITY)), hi = key_of(m) + 1;
-    u64 above = 0;
-    while (hi - lo > 1) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      const float f = float_of(mid);
-      const u64 s = mass([&](float x) { return x >= f; });
-      if ((double)s >= target) lo = mid; else hi = mid, above = s;
     }
-    const float f = float_of(lo);
-    // of the values equal to f, those in front of which less than the target lies
-    const double need = ceil((target - (double)above) / (double)weigh(f));
-    const int most = f == cut ? last : V - 1;
-    int equal = 0;
-    row.visit([&](int col, float (&x)[4], int) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) equal += clean(x[j]) == f && col + j <= most;
-    });
-    equal = block_reduce<NT>(equal, redi, AddOp());
-    last = most;
-    if (need < (double)equal) last = nth_equal(f, need < 1.0 ? 1 : (long)need);
-    cut = f;
+    if (by_p) {
+      if (all) {
+        u64 q = 0;
+        for (int i = tid; i < kBins; i += NT) q += s.bin.mass[i];
+        total = block_reduce<NT>(q, s.redu, AddOp());
+      }
+      const u64 target = share(total);
+      find_bin<NT, true>(s, target);
+      const int b = uniform(s.bin_at);
+      if (b < kBins) border(b, uniform(s.bin_mass), target, true);
+    }
   }
 
-  // ---- the draw: sums of a wave's chunk, in the order of the columns
-  const double floor_w = min_p > 1.0f ? 1.0 : (double)min_p;  // (NaN: no floor)
+  // ---- the draw, in the order of the columns: the weight of each wave's chunks, then the lane
   auto weight = [&](float x, int col) -> u64 {
     if (!kept(x, col)) return 0;
     const double q = weigh.real(x);
-    return q < floor_w ? 0 : (u64)(q * kOne + 0.5);
+    return q < floor_w ? 0 : weigh.whole(q);
   };
   u64 total = 0;
   row.visit([&](int col, float (&x)[4], int c) {
-    u64 s = 0;
+    u64 q = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s += weight(clean(x[j]), col + j);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (lane == 0) part[c * NW + w] = s;
-    total += s;
+    for (int j = 0; j < 4; ++j) q += weight(clean(x[j]), col + j);
+    if (__any(q != 0)) q = wave_reduce(q, AddOp());
+    total += q;
+    if (lane == 0) part[c * NW + w] = q;
   });
   if (lane != 0) total = 0;
-  total = block_reduce<NT>(total, redu, AddOp());
+  total = block_reduce<NT>(total, s.redu, AddOp());
   __syncthreads();
-  double u = (double)a.u[n];
-  if (!(u > 0.0)) u = 0.0;
-  const double at = u * (double)total;
-  u64 r = at < (double)total ? (u64)at : total - 1;
-  if (r >= total) r = total - 1;
+  const u64 r = place(total);
   if (w == 0) {  // the wave and chunk that holds it
     const int np = row.chunks() * NW, per = (np + 63) / 64;
-    u64 s = 0;
-    for (int i = lane * per; i < min((lane + 1) * per, np); ++i) s += part[i];
-    u64 upto = s;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const u64 x = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += x;
-    }
-    u64 before = upto - s;
-    if (r >= before && r < upto) {
+    u64 q = 0;
+    for (int i = lane * per; i < min((lane + 1) * per, np); ++i) q += part[i];
+    u64 before = wave_scan(q) - q;
+    if (r >= before && r < before + q) {
       int i = lane * per;
       while (r >= before + part[i]) before += part[i++];
-      found = i;
-      left = r - before;
+      s.chosen = i;
+      s.chosen_mass = r - before;
     }
   }
   __syncthreads();
-  const int fc = found / NW, fw = found % NW;
-  const u64 rr = left;
+  const int at = uniform(s.chosen), fc = at / NW, fw = at % NW;
+  const u64 rest = uniform(s.chosen_mass);
   if (w == fw)
     row.visit([&](int col, float (&x)[4], int c) {
       if (c != fc) return;
-      u64 q[4], s = 0;
+      u64 q[4], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s += q[j] = weight(clean(x[j]), col + j);
-      u64 upto = s;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += y;
-      }
-      u64 before = upto - s;
-      if (rr >= before && rr < upto) {
+      for (int j = 0; j < 4; ++j) sum += q[j] = weight(clean(x[j]), col + j);
+      u64 before = wave_scan(sum) - sum;
+      if (rest >= before && rest < before + sum) {
         int pick = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (rr >= before && rr < before + q[j]) pick = col + j;
+          if (rest >= before && rest < before + q[j]) pick = col + j;
           before += q[j];
         }
         a.out[n] = pick;
@@ -216,12 +432,26 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     });
 }
 
-void launch_filter_sample(const FilterArgs& a, hipStream_t s) {
-#define CALL(NTH, E)                                                         \
-  if (a.r.is_bf16) filter_sample_kernel<bf16, NTH, E><<<a.r.N, NTH, 0, s>>>(a); \
-  else filter_sample_kernel<float, NTH, E><<<a.r.N, NTH, 0, s>>>(a)
-  DCR_ROW_DISPATCH(a.r.V, CALL);
+template <typename T>
+static void launch_type(const FilterArgs& a, hipStream_t s) {
+  const int V = a.r.V;
+  auto lds = [&](int nt) { return (size_t)((V + nt * 4 - 1) / (nt * 4)) * nt * 4 * sizeof(T); };
+#define CALL(NTH, E, LDS) filter_sample_kernel<T, NTH, E><<<a.r.N, NTH, LDS, s>>>(a)
+  if (V <= 256) CALL(64, 4, 0);
+  else if (V <= 1024) CALL(64, 16, 0);
+  else if (lds(256) <= 32768) CALL(256, -1, lds(256));
+  else if (lds(1024) <= 131072) {
+    if (lds(1024) > 32768)
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&filter_sample_kernel<T, 1024, -1>),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, 131072);
+    CALL(1024, -1, lds(1024));
+  }
+  else CALL(1024, 0, 0);
 #undef CALL
+}
+
+void launch_filter_sample(const FilterArgs& a, hipStream_t s) {
+  if (a.r.is_bf16) launch_type<bf16>(a, s); else launch_type<float>(a, s);
 }
 
 }  // namespace dcr

@@ -2,16 +2,18 @@
 // temperature: what a teacher records for distillation.  Order: value descending, ties by the
 // lowest index; NaN counts as -inf in the order and makes the log-sum-exp NaN.
 //
-// One workgroup a row.  The row is read once into registers; the k-th largest value is found by
-// bisection over the order-preserving keys of the values (counts over registers), the k chosen
-// entries meet in LDS and each finds its place by counting.
+// One workgroup a row; the row is read once into registers, and that read is the bound.  Up to
+// 1024 columns (one wave) the k-th largest value is found by halving a range of values, with
+// counts by ballot.  Larger rows first find a value that at least k of them reach, from the maxima
+// of 1024 groups of columns; the some k entries that reach it meet in LDS.  Each collected entry
+// finds its place by counting those in front of it.
 #include "vocab_row.h"
 
 namespace dcr {
 
 namespace {
 
-__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }  // NaN -> -inf
+constexpr int kList = 1024;  // entries that meet in LDS; more (many equal values) are cut first
 
 }  // namespace
 
@@ -20,87 +22,83 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
                                                   float* __restrict__ values,
                                                   int* __restrict__ indices,
                                                   float* __restrict__ lse) {
+  constexpr bool kSmall = NT == 64 && EPT <= 16;
   __shared__ float redf[NT / 64];
   __shared__ int redi[NT / 64];
-  __shared__ float lv[kRowMaxK];
-  __shared__ int li[kRowMaxK], count;
+  constexpr int kCap = kSmall ? kRowMaxK : kList;
+  __shared__ float lv[kCap];
+  __shared__ int li[kCap], count;
+  __shared__ float gm[NT == 64 ? 1 : kGroups], reached;
   const long n = blockIdx.x;
   const int tid = threadIdx.x, V = r.V;
-  Row<T, NT, EPT> row(reinterpret_cast<const T*>(r.logits) + n * r.ld, V);
+  const float log2e_t = inv_t * 1.44269504088896341f;
+  const T* z = reinterpret_cast<const T*>(r.logits) + n * r.ld;
+  Row<T, NT, EPT> row(z, V);
 
   float m = -INFINITY;
-  int nan = 0;
   row.visit([&](int, float (&x)[4], int) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      nan |= x[j] != x[j];
-      m = fmaxf(m, x[j]);
-    }
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, x[j]);
   });
+  if (tid == 0) count = 0;
   m = block_reduce<NT>(m, redf, MaxOp());
-  nan = block_reduce<NT>(nan, redi, AddOp());
-  float sum = 0.f;
-  row.visit([&](int, float (&x)[4], int) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum += __expf((clean(x[j]) - m) * inv_t);
-  });
-  sum = block_reduce<NT>(sum, redf, AddOp());
-  if (tid == 0) {
-    lse[n] = nan ? __uint_as_float(0x7fc00000u)
-                 : (m == INFINITY || m == -INFINITY) ? m : m * inv_t + __logf(sum);
-    count = 0;
-  }
-
-  // count(>= lo) >= k > count(>= hi)
-  unsigned lo = key_of(-INFINITY), hi = key_of(m) + 1;
-  int above = 0, have = V;  // counts at hi and lo
-  while (hi - lo > 1 && have != k) {
-    const unsigned mid = lo + (hi - lo) / 2;
-    const float f = float_of(mid);
-    int c = 0;
+  if (m > -INFINITY && m < INFINITY) {
+    float sum = 0.f;
     row.visit([&](int, float (&x)[4], int) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c += x[j] >= f;
+      for (int j = 0; j < 4; ++j) sum += __builtin_amdgcn_exp2f((x[j] - m) * log2e_t);
     });
-    c = block_reduce<NT>(c, redi, AddOp());
-    if (c >= k) lo = mid, have = c; else hi = mid, above = c;
-  }
-  const float cut = float_of(lo);
-  int last = V - 1;  // entries equal to the cut are taken up to this column
-  if (have != k) {   // more of them than places: the lowest columns
-    const int need = k - above;
-    int a = -1, b = V - 1;  // count(== cut, column <= b) >= need > count(.., column <= a)
-    while (b - a > 1) {
-      const int mid = a + (b - a) / 2;
-      int c = 0;
-      row.visit([&](int col, float (&x)[4], int) {
+    sum = block_reduce<NT>(sum, redf, AddOp());  // (NaN where the row holds one)
+    if (tid == 0) lse[n] = m * inv_t + __logf(sum);
+  } else {
+    int nan = 0;
+    row.visit([&](int, float (&x)[4], int) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c += clean(x[j]) == cut && col + j <= mid;
-      });
-      c = block_reduce<NT>(c, redi, AddOp());
-      if (c >= need) b = mid; else a = mid;
-    }
-    last = b;
+      for (int j = 0; j < 4; ++j) nan |= x[j] != x[j];
+    });
+    nan = __syncthreads_or(nan);
+    if (tid == 0) lse[n] = nan ? __uint_as_float(0x7fc00000u) : m;
   }
-  __syncthreads();
-  row.visit([&](int col, float (&x)[4], int) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float y = clean(x[j]);
-      if (y > cut || (y == cut && col + j <= last)) {
-        const int at = atomicAdd(&count, 1);
-        if (at < kRowMaxK) lv[at] = y, li[at] = col + j;
-      }
+
+  int c = 0;  // collected entries
+  if constexpr (!kSmall) {
+    const float f = reached_by<NT>(row, gm, &reached, k);
+    if (f > -INFINITY) {
+      collect<NT>(row, lv, li, &count, kList, [&](float x, int) { return x >= f; });
+      c = uniform(count);
     }
-  });
-  __syncthreads();
-  for (int i = tid; i < k; i += NT) {
+  }
+  if (c < k || c > kList) {
+    // hardly ever for the long rows: they are read again rather than hold registers for it
+    auto again = [&] {
+      if constexpr (kSmall) return row;
+      else return Row<T, NT, 0>(z, V);
+    }();
+    float low = INFINITY;
+    again.visit([&](int, float (&x)[4], int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (x[j] > -INFINITY) low = fminf(low, x[j]);
+    });
+    low = block_reduce<NT>(low, redf, MinOp());
+    if (!kSmall && tid == 0) count = 0;
+    const Cut cut = cut_by_count<NT>(again, redi, m, low, k);
+    __syncthreads();
+    collect<NT>(again, lv, li, &count, k, [&](float x, int col) {
+      return x > cut.value || (x == cut.value && col <= cut.last);
+    });
+    c = k;
+  }
+  for (int i = tid; i < c; i += NT) {
     const float y = lv[i];
-    const int c = li[i];
+    const int col = li[i];
     int at = 0;
-    for (int j = 0; j < k; ++j) at += lv[j] > y || (lv[j] == y && li[j] < c);
-    values[n * k + at] = y;
-    indices[n * k + at] = c;
+#pragma unroll 8
+    for (int j = 0; j < c; ++j) at += lv[j] > y || (lv[j] == y && li[j] < col);
+    if (at < k) {
+      values[n * k + at] = y;
+      indices[n * k + at] = col;
+    }
   }
 }
 

@@ -198,6 +198,7 @@ def _cpu_distill_xent(logits, values, indices, lse, targets, alpha, tau, scale, 
         _check_rows(targets, logits, torch.int32, (n,), "targets")
         skip = skip | (targets < 0) | (targets >= v)
     z = torch.where(skip[:, None], 0.0, z)
+    z = z - torch.where(skip[:, None], 0.0, z.max(1, keepdim=True).values)
     logp = torch.log_softmax(z / tau, 1)
     t = torch.where(here, values / tau, -math.inf)
     some = ~torch.isneginf(t).all(1)

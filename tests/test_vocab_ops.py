@@ -239,6 +239,31 @@ def test_distill_odd_records(V, dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tau", [0.5, 2.0])
+def test_distill_lowest_values(tau, dtype, dev):
+    """Masks of the type's lowest value, and rows of nothing else: those are uniform."""
+    N, V, k = 3, 300, 4
+    low = torch.finfo(dtype).min
+    z = rows(N, V, dtype, dev)
+    values, indices, lse = record(z, k, tau)
+    z[0] = low
+    masked = torch.ones(V, dtype=torch.bool, device=dev)
+    masked[indices[1].long()] = False
+    z[1, masked] = low
+    y = indices[:, 0].contiguous()
+    loss, row, grad = O.distill_xent(z, values, indices, top_lse=None, targets=y, alpha=0.5,
+                                     temperature=tau)
+    half = 2.0 ** -8 if dtype == BF16 else 0.0
+    zs = z.double().cpu()
+    zs[0] = 0.0  # the same distribution
+    want, gwant = reference_distill(zs, values, indices, None, y, 0.5, tau, 1.0 / N)
+    assert ((row.double().cpu() - want).abs() <= 256 * U * 30 * (tau * tau + 1)).all(), (row, want)
+    tol = 256 * U * (tau + 1)
+    assert ((grad.double().cpu() - gwant).abs() <= tol + half * (gwant.abs() + tol)).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_distill_infinite_and_nan(dev):
     z = rows(4, 70, F32, dev)
     values, indices, lse = record(z, 4, 1.0)
