@@ -586,6 +586,7 @@ void launch_sample_step(const SampleArgs& a, hipStream_t s);
 // strides (in elements) along T and B; states are [B, H] contiguous fp32.
 constexpr int kLinrecSteps = 8;  // consecutive steps a wave holds in registers
 struct LinrecPlan {
+  int vec;            // neighbouring channels a lane
   int waves;          // waves of a workgroup; a tile is waves * kLinrecSteps steps
   int tiles;          // tiles of the time axis
   int segs, tiles_per_seg;  // segments of the time axis (1: no summary launch)

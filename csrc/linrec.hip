@@ -71,9 +71,10 @@ __device__ __forceinline__ void gates(float f, float& keep, float& take) {
   keep = f >= 0.f ? r : t * r;
   take = f >= 0.f ? t * r : r;
 }
-// a h + b, where a factor of zero (a start) lets nothing of h through, not even a NaN
+// a h + b; with MARKS a factor of zero (a start) lets nothing of h through, not even a NaN
+template <bool MARKS>
 __device__ __forceinline__ float step_(float a, float h, float b) {
-  return a == 0.f ? b : __builtin_fmaf(a, h, b);
+  return MARKS && a == 0.f ? b : __builtin_fmaf(a, h, b);
 }
 
 struct Lane {  // one lane's VEC channels
@@ -82,6 +83,13 @@ struct Lane {  // one lane's VEC channels
   long c;  // flattened channel b * H + h
   int h;
 };
+
+// The second launch takes the segments the other way round: what the first read last is still
+// in the last-level cache.
+template <bool SUMMARY>
+__device__ __forceinline__ int segment_of() {
+  return SUMMARY ? blockIdx.y : gridDim.y - 1 - blockIdx.y;
+}
 
 template <int VEC>
 __device__ __forceinline__ Lane lane_of(const LinrecArgs& p, int lane) {
@@ -100,11 +108,12 @@ __device__ __forceinline__ Lane lane_of(const LinrecArgs& p, int lane) {
 
 }  // namespace
 
-// SUMMARY: only the segment's pair (A, B) is formed (p.sumA / p.sumB).
-template <typename T, int VEC, int W, bool SUMMARY>
+// MARKS: lengths or starts are given.  SUMMARY: only the segment's pair (A, B) is formed
+// (p.sumA / p.sumB).
+template <typename T, int VEC, int W, bool MARKS, bool SUMMARY>
 __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
   __shared__ float sA[2][W][64 * VEC], sB[2][W][64 * VEC];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, seg = blockIdx.y;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, seg = segment_of<SUMMARY>();
   const Lane l = lane_of<VEC>(p, lane);
   const T* x = reinterpret_cast<const T*>(p.x) + l.b * p.x_b + l.h;
   const T* f = reinterpret_cast<const T*>(p.f) + l.b * p.f_b + l.h;
@@ -119,10 +128,11 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
     pa[j] = 1.f;
   }
   if (!SUMMARY)
+#pragma unroll 4
     for (int s = 0; s < seg; ++s)
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        carry[j] = step_(p.sumA[s * BH + l.c + j], carry[j], p.sumB[s * BH + l.c + j]);
+        carry[j] = step_<MARKS>(p.sumA[s * BH + l.c + j], carry[j], p.sumB[s * BH + l.c + j]);
 
   const int tile1 = min((seg + 1) * p.tiles_per_seg, p.tiles);
   int buf = 0;
@@ -141,14 +151,14 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       const bool live = t0 + i < l.len;
-      const bool start = st && st[(long)min(t0 + i, p.T - 1) * p.starts_t];
+      const bool start = MARKS && st && st[(long)min(t0 + i, p.T - 1) * p.starts_t];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float keep, take;
         gates(a[i][j], keep, take);
         a[i][j] = !live ? 1.f : start ? 0.f : keep;
         b[i][j] = live ? take * b[i][j] : 0.f;
-        B[j] = step_(a[i][j], B[j], b[i][j]);
+        B[j] = step_<MARKS>(a[i][j], B[j], b[i][j]);
         A[j] *= a[i][j];
       }
     }
@@ -170,7 +180,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
       for (int j = 0; j < VEC; ++j) {
         if (ww == w) h[j] = carry[j];
         const float aa = sA[buf][ww][lane * VEC + j];
-        carry[j] = step_(aa, carry[j], sB[buf][ww][lane * VEC + j]);
+        carry[j] = step_<MARKS>(aa, carry[j], sB[buf][ww][lane * VEC + j]);
         if (SUMMARY) pa[j] *= aa;
       }
     if (!SUMMARY) {
@@ -179,7 +189,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
         float y[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          h[j] = step_(a[i][j], h[j], b[i][j]);
+          h[j] = step_<MARKS>(a[i][j], h[j], b[i][j]);
           y[j] = t0 + i < l.len ? h[j] : 0.f;
         }
         if (l.on && t0 + i < p.T) store_row<T, VEC>(out + (long)(t0 + i) * p.h_t, y);
@@ -202,10 +212,10 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
 
 // Time runs backwards: e, the gradient with respect to the state in front of a stretch, is
 // A e_out + G with the same A.  SUMMARY forms the segment's (A, G) from f and dh alone.
-template <typename T, int VEC, int W, bool SUMMARY>
+template <typename T, int VEC, int W, bool MARKS, bool SUMMARY>
 __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
   __shared__ float sA[2][W][64 * VEC], sB[2][W][64 * VEC], sG[2][W][64 * VEC];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, seg = blockIdx.y;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, seg = segment_of<SUMMARY>();
   const Lane l = lane_of<VEC>(p, lane);
   const T* x = reinterpret_cast<const T*>(p.x) + l.b * p.x_b + l.h;
   const T* f = reinterpret_cast<const T*>(p.f) + l.b * p.f_b + l.h;
@@ -222,10 +232,11 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
     pa[j] = 1.f;
   }
   if (!SUMMARY)
+#pragma unroll 4
     for (int s = (int)gridDim.y - 1; s > seg; --s)
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        e[j] = step_(p.sumA[s * BH + l.c + j], e[j], p.sumB[s * BH + l.c + j]);
+        e[j] = step_<MARKS>(p.sumA[s * BH + l.c + j], e[j], p.sumB[s * BH + l.c + j]);
 
   const int tile1 = min((seg + 1) * p.tiles_per_seg, p.tiles);
   int buf = 0;
@@ -249,14 +260,14 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       const bool live = t0 + i < l.len;
-      if (st && live && st[(long)(t0 + i) * p.starts_t]) cut |= 1u << i;
+      if (MARKS && st && live && st[(long)(t0 + i) * p.starts_t]) cut |= 1u << i;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         gates(keep[i][j], keep[i][j], take[i][j]);
         if (!live) keep[i][j] = 1.f, take[i][j] = 0.f, g[i][j] = 0.f;
         if (!live && !SUMMARY) xv[i][j] = 0.f;
-        const float a = (cut >> i & 1) ? 0.f : keep[i][j];
-        if (!SUMMARY) B[j] = step_(a, B[j], take[i][j] * xv[i][j]);
+        const float a = (MARKS && (cut >> i & 1)) ? 0.f : keep[i][j];
+        if (!SUMMARY) B[j] = step_<MARKS>(a, B[j], take[i][j] * xv[i][j]);
         A[j] *= a;
       }
     }
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
     for (int i = kC - 1; i >= 0; --i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        G[j] = (cut >> i & 1) ? 0.f : keep[i][j] * (g[i][j] + G[j]);
+        G[j] = (MARKS && (cut >> i & 1)) ? 0.f : keep[i][j] * (g[i][j] + G[j]);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       sA[buf][w][lane * VEC + j] = A[j];
@@ -278,7 +289,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
         if (ww < w)
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
-            h[j] = step_(sA[buf][ww][lane * VEC + j], h[j], sB[buf][ww][lane * VEC + j]);
+            h[j] = step_<MARKS>(sA[buf][ww][lane * VEC + j], h[j], sB[buf][ww][lane * VEC + j]);
     float ein[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) ein[j] = e[j];
@@ -288,7 +299,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
       for (int j = 0; j < VEC; ++j) {
         if (ww == w) ein[j] = e[j];
         const float aa = sA[buf][ww][lane * VEC + j];
-        e[j] = step_(aa, e[j], sG[buf][ww][lane * VEC + j]);
+        e[j] = step_<MARKS>(aa, e[j], sG[buf][ww][lane * VEC + j]);
         if (SUMMARY) pa[j] *= aa;
       }
     if (!SUMMARY) {
@@ -297,7 +308,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
       for (int i = 0; i < kC; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          hp[i][j] = (cut >> i & 1) ? 0.f : h[j];
+          hp[i][j] = (MARKS && (cut >> i & 1)) ? 0.f : h[j];
           h[j] = __builtin_fmaf(keep[i][j], hp[i][j], take[i][j] * xv[i][j]);
         }
 #pragma unroll
@@ -309,7 +320,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
           const float cg = take[i][j] * gi;
           ox[j] = t0 + i < l.len ? cg : 0.f;
           of[j] = t0 + i < l.len ? keep[i][j] * cg * (hp[i][j] - xv[i][j]) : 0.f;
-          ein[j] = (cut >> i & 1) ? 0.f : keep[i][j] * gi;
+          ein[j] = (MARKS && (cut >> i & 1)) ? 0.f : keep[i][j] * gi;
         }
         if (l.on && t0 + i < p.T) {
           store_row<T, VEC>(dx + (long)(t0 + i) * p.dx_t, ox);
@@ -357,45 +368,60 @@ __global__ void __launch_bounds__(256) linrec_step_kernel(LinrecArgs p) {
 
 namespace {
 
-int vec_of(int H) { return H % 4 == 0 ? 4 : H % 2 == 0 ? 2 : 1; }
-
-template <typename T, int VEC, int W>
+template <typename T, int VEC, int W, bool MARKS>
 void run_seq(LinrecArgs& p, bool bwd, hipStream_t s) {
   const long groups = (long)p.B * (p.H / VEC);
   const dim3 grid((unsigned)((groups + 63) / 64), (unsigned)p.segs), block(64 * W);
   if (bwd) {
-    if (p.segs > 1) linrec_bwd_kernel<T, VEC, W, true><<<grid, block, 0, s>>>(p);
-    linrec_bwd_kernel<T, VEC, W, false><<<grid, block, 0, s>>>(p);
+    if (p.segs > 1) linrec_bwd_kernel<T, VEC, W, MARKS, true><<<grid, block, 0, s>>>(p);
+    linrec_bwd_kernel<T, VEC, W, MARKS, false><<<grid, block, 0, s>>>(p);
   } else {
-    if (p.segs > 1) linrec_fwd_kernel<T, VEC, W, true><<<grid, block, 0, s>>>(p);
-    linrec_fwd_kernel<T, VEC, W, false><<<grid, block, 0, s>>>(p);
+    if (p.segs > 1) linrec_fwd_kernel<T, VEC, W, MARKS, true><<<grid, block, 0, s>>>(p);
+    linrec_fwd_kernel<T, VEC, W, MARKS, false><<<grid, block, 0, s>>>(p);
   }
 }
 
-template <typename T>
-void run_type(LinrecArgs& p, bool bwd, int vec, int waves, hipStream_t s) {
-  if (waves == 16) {
-    if (vec >= 2) run_seq<T, 2, 16>(p, bwd, s); else run_seq<T, 1, 16>(p, bwd, s);
-  } else {
-    if (vec == 4) run_seq<T, 4, 4>(p, bwd, s);
-    else if (vec == 2) run_seq<T, 2, 4>(p, bwd, s);
-    else run_seq<T, 1, 4>(p, bwd, s);
+template <typename T, int W>
+void run_type(LinrecArgs& p, bool bwd, int vec, hipStream_t s) {
+  const bool marks = p.lengths || p.starts;
+#define LR(VV) \
+  if (marks) run_seq<T, VV, W, true>(p, bwd, s); else run_seq<T, VV, W, false>(p, bwd, s)
+  if constexpr (W == 4) {
+    if (vec == 4) {
+      LR(4);
+      return;
+    }
   }
+  if (vec == 2) { LR(2); } else { LR(1); }
+#undef LR
 }
 
 }  // namespace
 
-// Waves a workgroup and segments of the time axis.  
+// Channels a lane, waves a workgroup and segments of the time axis, from the sizes alone (the
+// backward has to find the forward's tiles).  Measured on one MI355X, forward / backward us:
+//  * the widest loads that leave some 192 workgroups, else single channels: 25600 channels, 1024
+//    steps, bf16: 51 / 68 with two channels a lane, 52 / 78 with one, 108 / 135 with four;
+//  * four waves where a lane has four channels (128 steps of 256 x 512 bf16: 25 / 37, with eight
+//    25 / 42; 16384 steps of 4 x 1000, padded documents: 165 / 232 against 184 / 275), else eight:
+//    longer tiles, fewer of them (4096 steps of 512 channels: 12.6 / 18.3, with four 14.5 / 21.0);
+//  * segments where even single channels leave fewer workgroups and there are 512 steps or more,
+//    although x, f and dh are then read twice (4096 steps of 512 channels: 12.6 / 18.3 with 64
+//    segments, 41 / 56 with 16); for 200 steps of 6400 channels one segment takes 8.7 / 12.0, eight
+//    11.0 / 12.8.  At most 64: each workgroup folds the pairs in front of its segment.
 LinrecPlan linrec_plan(int T, int B, int H) {
-  LinrecPlan q;
-  const int vec = vec_of(H);
-  const long wgs = ((long)B * (H / vec) + 63) / 64 + ((long)B * H == 0);  // at least one
-  q.waves = wgs >= 256 || T <= 4 * kC ? 4 : 16;
+  LinrecPlan q{};
+  auto wgs = [&](int vec) { return ((long)B * (H / vec) + 63) / 64; };
+  const int widest = H % 4 == 0 ? 4 : H % 2 == 0 ? 2 : 1;
+  const bool split = T >= 512 && wgs(1) < 192;
+  const long cuts = split ? (T / 64 < 64 ? T / 64 : 64) : 1;
+  q.vec = widest;
+  while (q.vec > 1 && wgs(q.vec) * cuts < (split ? 512 : 192)) q.vec /= 2;
+  const long n = wgs(q.vec) > 0 ? wgs(q.vec) : 1;
+  q.waves = T <= 32 || q.vec == 4 ? 4 : 8;
   q.tiles = (T + q.waves * kC - 1) / (q.waves * kC);
-  long segs = wgs >= 512 ? 1 : (512 + wgs - 1) / wgs;
+  long segs = split ? ((q.waves == 4 ? 1024 : 512) + n - 1) / n : 1;
   if (segs > 64) segs = 64;
-  if (segs > q.tiles) segs = q.tiles;
-  if (segs < 1) segs = 1;
   q.tiles_per_seg = (int)((q.tiles + segs - 1) / segs);
   if (q.tiles_per_seg < 1) q.tiles_per_seg = 1;
   q.segs = (q.tiles + q.tiles_per_seg - 1) / q.tiles_per_seg;
@@ -408,14 +434,15 @@ void launch_linrec(LinrecArgs p, bool is_bf16, bool bwd, hipStream_t s) {
   p.tiles = q.tiles;
   p.tiles_per_seg = q.tiles_per_seg;
   p.segs = q.segs;
-  if (is_bf16)
-    run_type<bf16>(p, bwd, vec_of(p.H), q.waves, s);
-  else
-    run_type<float>(p, bwd, vec_of(p.H), q.waves, s);
+  if (is_bf16) {
+    if (q.waves == 4) run_type<bf16, 4>(p, bwd, q.vec, s); else run_type<bf16, 8>(p, bwd, q.vec, s);
+  } else {
+    if (q.waves == 4) run_type<float, 4>(p, bwd, q.vec, s); else run_type<float, 8>(p, bwd, q.vec, s);
+  }
 }
 
 void launch_linrec_step(const LinrecArgs& p, bool is_bf16, hipStream_t s) {
-  const int vec = vec_of(p.H);
+  const int vec = p.H % 4 == 0 ? 4 : p.H % 2 == 0 ? 2 : 1;
   const unsigned nb = (unsigned)(((long)p.B * (p.H / vec) + 255) / 256);
 #define LS(TT, VV) linrec_step_kernel<TT, VV><<<nb, 256, 0, s>>>(p)
   if (is_bf16) {
