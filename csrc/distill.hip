@@ -21,8 +21,6 @@ namespace dcr {
 template <typename T, typename G, int NT, int EPT>
 __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   constexpr int kE = NT < kRowMaxK ? kRowMaxK / NT : 1;  // entries a thread
-  constexpr bool kKeep = EPT > 0 && EPT <= 32;  // room for the exponentials beside the row
-  constexpr int kKept = kKeep ? EPT / 4 : 1;
   extern __shared__ unsigned bits[];
   __shared__ float red[(3 + 5 + 2) * (NT / 64)];
   __shared__ int ei[kRowMaxK], twice;
@@ -85,11 +83,30 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
 
   // ---- maxima: of the rest, of the entries' z and t
   float top[3] = {-INFINITY, -INFINITY, -INFINITY};
+  // sums at T and at 1: of the rest, of the entries' z; and of the entries' t
+  float sum[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const float (&x)[4], float over) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum[0] += __builtin_amdgcn_exp2f((x[j] - over) * c_t);
+      if (two) sum[1] += __builtin_amdgcn_exp2f((x[j] - over) * c_1);
+    }
+  };
   row.visit([&](int col, float (&x)[4], int) {
     rest_of(x, col);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top[0] = fmaxf(top[0], x[j]);
+    const float big = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    if constexpr (EPT > 0) {
+      top[0] = fmaxf(top[0], big);
+    } else {  // one reading for both: each thread's sums are over its own maximum so far
+      if (big > top[0]) {
+        sum[0] *= __builtin_amdgcn_exp2f((top[0] - big) * c_t);
+        sum[1] *= __builtin_amdgcn_exp2f((top[0] - big) * c_1);
+        top[0] = big;
+      }
+      add(x, top[0] == -INFINITY ? 0.f : top[0]);
+    }
   });
+  const float mine = top[0];
 #pragma unroll
   for (int e = 0; e < kE; ++e) {
     top[1] = fmaxf(top[1], z_e[e]);
@@ -98,24 +115,12 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   block_reduce_each<NT, 3>(top, red, MaxOp());
   const float mr = top[0], mk = top[1], mt = top[2], m = fmaxf(mr, mk);
   const float mr0 = mr == -INFINITY ? 0.f : mr;  // (an empty rest sums to 0)
-
-  // ---- sums at T and at 1: of the rest, of the entries' z; and of the entries' t
-  float sum[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-  float et[kKept][4], e1[kKept][4];
-  row.visit([&](int col, float (&x)[4], int c) {
-    rest_of(x, col);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d = x[j] - mr0, p = __builtin_amdgcn_exp2f(d * c_t);
-      sum[0] += p;
-      if (kKeep) et[kKeep ? c : 0][j] = p;
-      if (two) {
-        const float p1 = __builtin_amdgcn_exp2f(d * c_1);
-        sum[1] += p1;
-        if (kKeep) e1[kKeep ? c : 0][j] = p1;
-      }
-    }
-  });
+  if constexpr (EPT > 0) {
+    row.visit([&](int, float (&x)[4], int) { add(x, mr0); });
+  } else if (mine > -INFINITY) {
+    sum[0] *= __builtin_amdgcn_exp2f((mine - mr) * c_t);
+    sum[1] *= __builtin_amdgcn_exp2f((mine - mr) * c_1);
+  }
 #pragma unroll
   for (int e = 0; e < kE; ++e) {
     if (first[e] && z_e[e] != -INFINITY) {
@@ -174,14 +179,9 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     float g[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (kKeep) {
-        g[j] = ft * et[kKeep ? c : 0][j];
-        if (two) g[j] += f1 * e1[kKeep ? c : 0][j];
-      } else {
-        const float d = x[j] - mr0;
-        g[j] = ft * __builtin_amdgcn_exp2f(d * c_t);
-        if (two) g[j] += f1 * __builtin_amdgcn_exp2f(d * c_1);
-      }
+      const float d = x[j] - mr0;
+      g[j] = ft * __builtin_amdgcn_exp2f(d * c_t);
+      if (two) g[j] += f1 * __builtin_amdgcn_exp2f(d * c_1);
     }
     if (c == cy)
 #pragma unroll
@@ -224,18 +224,38 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const float* __restri
   if (threadIdx.x == 0) out[0] = s * scale;
 }
 
-void launch_distill(const DistillArgs& a, hipStream_t s) {
+// Workgroup and registers for N rows of V columns.  One wave takes a row of up to 1024 columns: no
+// barriers, and many rows a CU.  Up to 16384 columns, few rows get more threads, which is faster for
+// the row, and many get smaller workgroups, whose loads and computations overlap each other's
+// (fp32: 256 x 8192 7.8 us with 512 threads, 14.8 with 128; 32768 x 8192 343 with 128, 374 with 256).
+// Past 32768 the registers are too few for two workgroups a CU, and a row is read twice instead
+// (1024 x 65536 bf16: 101 us, 115 from registers).
+template <typename T, typename G>
+static void launch_types(const DistillArgs& a, hipStream_t s) {
   const size_t lds = (size_t)((a.r.V + 31) / 32) * 4;
-#define CALL(NTH, E)                                                             \
-  if (a.r.is_bf16) {                                                             \
-    if (a.grad_bf16) distill_kernel<bf16, bf16, NTH, E><<<a.r.N, NTH, lds, s>>>(a); \
-    else distill_kernel<bf16, float, NTH, E><<<a.r.N, NTH, lds, s>>>(a);         \
-  } else {                                                                       \
-    if (a.grad_bf16) distill_kernel<float, bf16, NTH, E><<<a.r.N, NTH, lds, s>>>(a); \
-    else distill_kernel<float, float, NTH, E><<<a.r.N, NTH, lds, s>>>(a);        \
-  }
-  if (a.r.N > 0) DCR_ROW_DISPATCH(a.r.V, CALL);
+  const int V = a.r.V;
+  const bool many = a.r.N >= 1024;
+#define CALL(NTH, E) distill_kernel<T, G, NTH, E><<<a.r.N, NTH, lds, s>>>(a)
+  if (V <= 256) CALL(64, 4);
+  else if (V <= 1024) CALL(64, 16);
+  else if (V <= 4096) CALL(256, 16);
+  else if (V <= 8192 && many) CALL(128, 64);
+  else if (V <= 8192) CALL(512, 16);
+  else if (V <= 16384 && many) CALL(256, 64);
+  else if (V <= 16384) CALL(512, 32);
+  else if (V <= 32768) CALL(512, 64);
+  else CALL(1024, 0);
 #undef CALL
+}
+
+void launch_distill(const DistillArgs& a, hipStream_t s) {
+  if (a.r.N > 0) {
+    if (a.r.is_bf16) {
+      if (a.grad_bf16) launch_types<bf16, bf16>(a, s); else launch_types<bf16, float>(a, s);
+    } else {
+      if (a.grad_bf16) launch_types<float, bf16>(a, s); else launch_types<float, float>(a, s);
+    }
+  }
   if (a.loss) distill_sum_kernel<<<1, 1024, 0, s>>>(a.row_loss, a.r.N, a.scale, a.loss);
 }
 

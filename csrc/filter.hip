@@ -68,12 +68,11 @@ struct Work {  // LDS of one workgroup
   float redf[NT / 64];
   int redi[NT / 64];
   u64 redu[NT / 64];
-  float lv[kCap];
-  int li[kCap];
+  alignas(16) Entry list[kCap];
   u64 lw[kCap];
   union {
     struct { u64 mass[kBins]; int count[kBins]; } bin;
-    struct { float v[kRowMaxK]; int i[kRowMaxK]; u64 w[kRowMaxK]; } top;  // ordered entries
+    struct { Entry e[kRowMaxK]; u64 w[kRowMaxK]; } top;  // ordered entries
     float gm[NT == 64 ? 1 : kGroups];
   };
   int n, chosen, chosen_last;
@@ -184,7 +183,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     if constexpr (NT != 64) {
       const float f = reached_by<NT>(row, s.gm, &s.reached, want);
       // (entries of -inf weigh nothing: fewer than `want` others are all that is needed)
-      collect<NT>(row, s.lv, s.li, &s.n, kCap, [&](float x, int) {
+      collect<NT>(row, s.list, &s.n, kCap, [&](float x, int) {
         return x >= f && x > -INFINITY;
       });
       c = uniform(s.n);
@@ -193,20 +192,17 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       const Cut cut = cut_by_count<NT>(row, s.redi, m, low, want);
       if (tid == 0) s.n = 0;
       __syncthreads();
-      collect<NT>(row, s.lv, s.li, &s.n, kCap, [&](float x, int col) {
+      collect<NT>(row, s.list, &s.n, kCap, [&](float x, int col) {
         return x > -INFINITY && (x > cut.value || (x == cut.value && col <= cut.last));
       });
       c = uniform(s.n);
     }
     for (int i = tid; i < c; i += NT) {
-      const float y = s.lv[i];
-      const int col = s.li[i];
-      int at = 0;
-      for (int j = 0; j < c; ++j) at += s.lv[j] > y || (s.lv[j] == y && s.li[j] < col);
+      const Entry mine = s.list[i];
+      const int at = place_of(s.list, c, mine);
       if (at < want) {
-        s.top.v[at] = y;
-        s.top.i[at] = col;
-        s.top.w[at] = weigh(y);
+        s.top.e[at] = mine;
+        s.top.w[at] = weigh(value_of(mine));
       }
     }
     c = min(c, want);
@@ -229,7 +225,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       for (int i = 0; i < kPer; ++i) {
         const int at = lane * kPer + i;
         const bool in = at < c && before < target &&
-                        (at == 0 || !(weigh.real(s.top.v[at]) < floor_w));
+                        (at == 0 || !(weigh.real(value_of(s.top.e[at])) < floor_w));
         before += q[i];
         if (in) kept = at + 1, mass += q[i];
       }
@@ -241,12 +237,12 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     c = uniform(s.chosen);
     const u64 r = place(s.chosen_total);
     for (int i = tid; i < c; i += NT) {  // running weights in the order of the indices
-      const int col = s.top.i[i];
+      const unsigned col = (unsigned)s.top.e[i];  // (its complement: larger for lower columns)
       const u64 mine = s.top.w[i];
       u64 before = 0;
-      for (int j = 0; j < c; ++j)
-        if (s.top.i[j] < col) before += s.top.w[j];
-      if (r >= before && r < before + mine) a.out[n] = col;
+#pragma unroll 4
+      for (int j = 0; j < c; ++j) before += (unsigned)s.top.e[j] > col ? s.top.w[j] : 0;
+      if (r >= before && r < before + mine) a.out[n] = (int)~col;
     }
     return;
   }
@@ -285,23 +281,27 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     auto border = [&](int b, u64 in_front, u64 target, bool by_mass) {
       if (tid == 0) s.n = 0;
       __syncthreads();
-      collect<NT>(row, s.lv, s.li, &s.n, kCap, [&](float x, int col) {
+      collect<NT>(row, s.list, &s.n, kCap, [&](float x, int col) {
         return x > -INFINITY && (x == m ? 0 : bin_of(x)) == b && kept(x, col);
       });
       const int c = uniform(s.n);
       if (c <= kCap) {
-        for (int i = tid; i < c; i += NT) s.lw[i] = weigh(s.lv[i]);
+        for (int i = tid; i < c; i += NT) s.lw[i] = weigh(value_of(s.list[i]));
         __syncthreads();
         for (int i = tid; i < c; i += NT) {
-          const float y = s.lv[i];
-          const int col = s.li[i];
-          u64 count = 0, mass = 0;
-          for (int j = 0; j < c; ++j)
-            if (s.lv[j] > y || (s.lv[j] == y && s.li[j] < col)) ++count, mass += s.lw[j];
-          const u64 before = in_front + (by_mass ? mass : count);
+          const Entry mine = s.list[i];
+          int count = 0;
+          u64 mass = 0;
+#pragma unroll 4
+          for (int j = 0; j < c; ++j) {
+            const bool front = s.list[j] > mine;
+            count += front;
+            mass += front ? s.lw[j] : 0;
+          }
+          const u64 before = in_front + (by_mass ? mass : (u64)count);
           if (before < target && target <= before + (by_mass ? s.lw[i] : 1)) {
-            s.chosen_value = y;
-            s.chosen_last = col;
+            s.chosen_value = value_of(mine);
+            s.chosen_last = column_of(mine);
             s.chosen_mass = mass + s.lw[i];
           }
         }

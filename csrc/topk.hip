@@ -26,8 +26,8 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
   __shared__ float redf[NT / 64];
   __shared__ int redi[NT / 64];
   constexpr int kCap = kSmall ? kRowMaxK : kList;
-  __shared__ float lv[kCap];
-  __shared__ int li[kCap], count;
+  __shared__ alignas(16) Entry list[kCap];
+  __shared__ int count;
   __shared__ float gm[NT == 64 ? 1 : kGroups], reached;
   const long n = blockIdx.x;
   const int tid = threadIdx.x, V = r.V;
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
   if constexpr (!kSmall) {
     const float f = reached_by<NT>(row, gm, &reached, k);
     if (f > -INFINITY) {
-      collect<NT>(row, lv, li, &count, kList, [&](float x, int) { return x >= f; });
+      collect<NT>(row, list, &count, kList, [&](float x, int) { return x >= f; });
       c = uniform(count);
     }
   }
@@ -84,33 +84,43 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
     if (!kSmall && tid == 0) count = 0;
     const Cut cut = cut_by_count<NT>(again, redi, m, low, k);
     __syncthreads();
-    collect<NT>(again, lv, li, &count, k, [&](float x, int col) {
+    collect<NT>(again, list, &count, k, [&](float x, int col) {
       return x > cut.value || (x == cut.value && col <= cut.last);
     });
     c = k;
   }
   for (int i = tid; i < c; i += NT) {
-    const float y = lv[i];
-    const int col = li[i];
-    int at = 0;
-#pragma unroll 8
-    for (int j = 0; j < c; ++j) at += lv[j] > y || (lv[j] == y && li[j] < col);
+    const Entry mine = list[i];
+    const int at = place_of(list, c, mine);
     if (at < k) {
-      values[n * k + at] = y;
-      indices[n * k + at] = col;
+      values[n * k + at] = value_of(mine);
+      indices[n * k + at] = column_of(mine);
     }
   }
 }
 
+// One wave takes a row of up to 1024 columns; longer rows get more threads before more registers,
+// and past 65536 columns are read again instead of held (1024 x 65536 bf16, k = 64: 74 us held, 92
+// read again).
+template <typename T>
+static void launch_type(const RowArgs& r, int k, float inv_t, float* values, int* indices,
+                        float* lse, hipStream_t s) {
+#define CALL(NTH, E) topk_kernel<T, NTH, E><<<r.N, NTH, 0, s>>>(r, k, inv_t, values, indices, lse)
+  if (r.V <= 256) CALL(64, 4);
+  else if (r.V <= 1024) CALL(64, 16);
+  else if (r.V <= 4096) CALL(256, 16);
+  else if (r.V <= 8192) CALL(256, 32);
+  else if (r.V <= 16384) CALL(512, 32);
+  else if (r.V <= 32768) CALL(512, 64);
+  else if (r.V <= 65536) CALL(1024, 64);
+  else CALL(1024, 0);
+#undef CALL
+}
+
 void launch_topk(const RowArgs& r, int k, float inv_t, float* values, int* indices, float* lse,
                  hipStream_t s) {
-#define CALL(NTH, E)                                                                         \
-  if (r.is_bf16)                                                                             \
-    topk_kernel<bf16, NTH, E><<<r.N, NTH, 0, s>>>(r, k, inv_t, values, indices, lse);        \
-  else                                                                                       \
-    topk_kernel<float, NTH, E><<<r.N, NTH, 0, s>>>(r, k, inv_t, values, indices, lse)
-  DCR_ROW_DISPATCH(r.V, CALL);
-#undef CALL
+  if (r.is_bf16) launch_type<bf16>(r, k, inv_t, values, indices, lse, s);
+  else launch_type<float>(r, k, inv_t, values, indices, lse, s);
 }
 
 }  // namespace dcr

@@ -62,6 +62,7 @@ struct Row {
   __device__ __forceinline__ void visit(F&& fn) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
+      if (c > 0 && c * NT * 4 >= V) continue;  // nobody's columns (wave-uniform)
       float v[4];
       forget(q[c]);
       widen<T>(q[c], v);
@@ -93,7 +94,7 @@ struct Row<T, NT, 0> {
   template <typename F>
   __device__ __forceinline__ void visit(F&& fn) {
     const int n = chunks();
-#pragma unroll 2
+#pragma unroll 4
     for (int c = 0; c < n; ++c) {
       const int col = (c * NT + (int)threadIdx.x) * 4;
       float v[4];
@@ -302,12 +303,20 @@ __device__ __forceinline__ Cut cut_by_count(R& row, int* red, float m, float low
   return cut;
 }
 
+// An entry as one number that orders as the entries do: larger values first, then lower columns.
+typedef unsigned long long Entry;
+__device__ __forceinline__ Entry entry_of(float x, int col) {
+  return (Entry)key_of(x) << 32 | (unsigned)~col;
+}
+__device__ __forceinline__ float value_of(Entry e) { return float_of((unsigned)(e >> 32)); }
+__device__ __forceinline__ int column_of(Entry e) { return (int)~(unsigned)e; }
+
 // Collects the row's entries with pred(value, column) in LDS, in no order; the count goes on past
 // `cap`, entries beyond it are not stored.  *count is zero before; a barrier follows.  A row in
 // registers is marked first (a bit a value), so a wave asks for its places once; others chunk by
 // chunk.
 template <int NT, typename R, typename P>
-__device__ __forceinline__ void collect(R& row, float* lv, int* li, int* count, int cap, P&& pred) {
+__device__ __forceinline__ void collect(R& row, Entry* list, int* count, int cap, P&& pred) {
   // whether the wave needs places, and the first of this lane's
   auto places = [&](int mine, int& at) {
     const int upto = wave_scan(mine), all = lane_value(upto, 63);
@@ -319,7 +328,7 @@ __device__ __forceinline__ void collect(R& row, float* lv, int* li, int* count, 
   };
   int at;
   auto put = [&](float x, int col, int at) {
-    if (at < cap) lv[at] = x, li[at] = col;
+    if (at < cap) list[at] = entry_of(x, col);
   };
   if constexpr (R::kChunks > 0) {
     constexpr int kWords = (R::kChunks + 7) / 8;
@@ -351,6 +360,21 @@ __device__ __forceinline__ void collect(R& row, float* lv, int* li, int* count, 
     });
   }
   __syncthreads();
+}
+
+// How many of the c entries in the list come in front of `mine`.  The list is 16-byte aligned and
+// has an entry to spare.
+__device__ __forceinline__ int place_of(const Entry* list, int c, Entry mine) {
+  struct alignas(16) Two { Entry a, b; };
+  const Two* two = reinterpret_cast<const Two*>(list);
+  int at = 0;
+#pragma unroll 4
+  for (int j = 0; j < c / 2; ++j) {
+    const Two q = two[j];
+    at += (q.a > mine) + (q.b > mine);
+  }
+  if (c & 1) at += list[c - 1] > mine;
+  return at;
 }
 
 // A value that at least k of the row reach and, unless many are equal, few more: the row is cut
@@ -414,18 +438,5 @@ __device__ __forceinline__ float reached_by(R& row, float* gm, float* out, int k
   __syncthreads();
   return uniform(*out);
 }
-
-// Workgroup and registers for rows of V columns.  One wave takes a row of up to 1024 columns: no
-// barriers, and many rows a CU; longer rows get more threads before more registers.
-#define DCR_ROW_DISPATCH(V, CALL)                \
-  do {                                           \
-    if ((V) <= 256) { CALL(64, 4); }             \
-    else if ((V) <= 1024) { CALL(64, 16); }      \
-    else if ((V) <= 4096) { CALL(256, 16); }     \
-    else if ((V) <= 8192) { CALL(256, 32); }     \
-    else if ((V) <= 32768) { CALL(512, 64); }    \
-    else if ((V) <= 65536) { CALL(1024, 64); }   \
-    else { CALL(1024, 0); }                      \
-  } while (0)
 
 }  // namespace dcr
