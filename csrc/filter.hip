@@ -33,13 +33,14 @@ __device__ __forceinline__ float of_row(const PerRow& p, long n) { return p.p ? 
 
 // 2^44 exp((x - m) / temperature), as a number and rounded.  2^f on [-1/2, 1/2] by its power
 // series to f^11 (the rest is below 2^-47); adding 2^52 leaves the rounded number in the low bits.
+// No branches: -inf (and the NaN of its product with a c of 0) ends at 2^-64, which rounds to 0, and a
+// row with +inf counts from 1e300, where all else ends there too.
 struct Weigh {
-  float m;
-  double c;  // log2(e) / temperature
+  double top, c;  // c = log2(e) / temperature
+  __device__ __forceinline__ Weigh(float m, float temp)
+      : top(m == INFINITY ? 1e300 : (double)m), c(fmax(1.4426950408889634 / (double)temp, 1e-280)) {}
   __device__ __forceinline__ double real(float x) const {
-    if (x == m) return 17592186044416.0;
-    if (x == -INFINITY || m == INFINITY) return 0.0;
-    const double y = fmax(((double)x - (double)m) * c, -64.0);
+    const double y = fmin(fmax(((double)x - top) * c, -64.0), 0.0);
     const double n = rint(y), f = y - n;
     double p = 4.4455382718708114e-10;  // ln(2)^k / k!, k = 11 .. 0
     p = fma(p, f, 7.0549116208011234e-09);
@@ -61,6 +62,21 @@ struct Weigh {
   __device__ __forceinline__ u64 operator()(float x) const { return whole(real(x)); }
 };
 
+// The threads of a workgroup take `c` entries together, kTeam threads each; f(entry, member)
+// returns a member's share of a sum, g(entry, sum) runs in every member.
+template <int NT, typename T, typename F, typename G>
+__device__ __forceinline__ void by_teams(int c, F&& f, G&& g) {
+  constexpr int kTeam = NT == 64 ? 1 : NT == 256 ? 2 : 4;
+  for (int i = threadIdx.x / kTeam; i - (int)threadIdx.x / kTeam < c; i += NT / kTeam) {
+    T x = i < c ? f(i, (int)threadIdx.x % kTeam, kTeam) : T(0);
+    if (kTeam > 1) x += dpp<0xB1>(x);
+    if (kTeam > 2) x += dpp<0x4E>(x);
+    if (i < c) g(i, x);
+  }
+}
+
+struct alignas(16) Weighed { Entry e; u64 w; };
+
 template <int NT>
 struct Work {  // LDS of one workgroup
   static constexpr int kBins = NT == 64 ? 256 : 1024;
@@ -72,7 +88,7 @@ struct Work {  // LDS of one workgroup
   u64 lw[kCap];
   union {
     struct { u64 mass[kBins]; int count[kBins]; } bin;
-    struct { Entry e[kRowMaxK]; u64 w[kRowMaxK]; } top;  // ordered entries
+    Weighed top[kRowMaxK];  // ordered entries
     float gm[NT == 64 ? 1 : kGroups];
   };
   int n, chosen, chosen_last;
@@ -159,7 +175,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     return;
   }
   low = block_reduce<NT>(low, s.redf, MinOp());
-  const Weigh weigh{m, 1.4426950408889634 / (double)temp};
+  const Weigh weigh(m, temp);
   const float top_p = uniform(of_row(a.top_p, n)), min_p = of_row(a.min_p, n);
   const int want = uniform(a.top_k ? a.top_k[n] : a.top_k_all);
   // (a NaN min_p: no floor)
@@ -197,14 +213,19 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       });
       c = uniform(s.n);
     }
-    for (int i = tid; i < c; i += NT) {
-      const Entry mine = s.list[i];
-      const int at = place_of(s.list, c, mine);
-      if (at < want) {
-        s.top.e[at] = mine;
-        s.top.w[at] = weigh(value_of(mine));
-      }
-    }
+    by_teams<NT, int>(
+        c,
+        [&](int i, int k, int K) {
+          const Entry mine = s.list[i];
+          const int part = ((c + K - 1) / K + 1) & ~1, from = k * part;  // pairs stay together
+          return place_of(s.list + from, max(0, min(c - from, part)), mine);
+        },
+        [&](int i, int at) {
+          if (at < want) {
+            const Entry mine = s.list[i];
+            s.top[at] = Weighed{mine, weigh(value_of(mine))};
+          }
+        });
     c = min(c, want);
     __syncthreads();
     if (w == 0) {
@@ -213,7 +234,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int at = lane * kPer + i;
-        q[i] = at < c ? s.top.w[at] : 0;
+        q[i] = at < c ? s.top[at].w : 0;
         sum += q[i];
       }
       u64 before = wave_scan(sum) - sum;
@@ -225,7 +246,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       for (int i = 0; i < kPer; ++i) {
         const int at = lane * kPer + i;
         const bool in = at < c && before < target &&
-                        (at == 0 || !(weigh.real(value_of(s.top.e[at])) < floor_w));
+                        (at == 0 || !(weigh.real(value_of(s.top[at].e)) < floor_w));
         before += q[i];
         if (in) kept = at + 1, mass += q[i];
       }
@@ -236,14 +257,21 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     __syncthreads();
     c = uniform(s.chosen);
     const u64 r = place(s.chosen_total);
-    for (int i = tid; i < c; i += NT) {  // running weights in the order of the indices
-      const unsigned col = (unsigned)s.top.e[i];  // (its complement: larger for lower columns)
-      const u64 mine = s.top.w[i];
-      u64 before = 0;
-#pragma unroll 4
-      for (int j = 0; j < c; ++j) before += (unsigned)s.top.e[j] > col ? s.top.w[j] : 0;
-      if (r >= before && r < before + mine) a.out[n] = (int)~col;
-    }
+    by_teams<NT, u64>(  // running weights in the order of the indices
+        c,
+        [&](int i, int k, int K) {
+          const unsigned col = (unsigned)s.top[i].e;  // (its complement: larger for lower columns)
+          u64 before = 0;
+#pragma unroll 8
+          for (int j = k; j < c; j += K) {
+            const Weighed q = s.top[j];
+            before += (unsigned)q.e > col ? q.w : 0;
+          }
+          return before;
+        },
+        [&](int i, u64 before) {
+          if (r >= before && r < before + s.top[i].w) a.out[n] = column_of(s.top[i].e);
+        });
     return;
   }
 
@@ -260,6 +288,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
     const float per = span > 0.f ? (float)kBins / span : 0.f;
     const bool clipped = !((m - low) * inv_t < 32.0f);
     auto bin_of = [&](float x) {
+      if (x == m) return 0;
       const float d = (m - x) * inv_t * per;  // falls with x, also as rounded
       return d < (float)(kBins - 1) ? (int)d : kBins - 1;
     };
@@ -269,7 +298,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (x[j] > -INFINITY) {
-          const int b = x[j] == m ? 0 : bin_of(x[j]);
+          const int b = bin_of(x[j]);
           const u64 q = weigh(x[j]);
           if (by_k) atomicAdd(&s.bin.count[b], 1);
           if (q) atomicAdd(&s.bin.mass[b], q);
@@ -282,34 +311,38 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       if (tid == 0) s.n = 0;
       __syncthreads();
       collect<NT>(row, s.list, &s.n, kCap, [&](float x, int col) {
-        return x > -INFINITY && (x == m ? 0 : bin_of(x)) == b && kept(x, col);
+        return x > -INFINITY && bin_of(x) == b && kept(x, col);
       });
       const int c = uniform(s.n);
       if (c <= kCap) {
         for (int i = tid; i < c; i += NT) s.lw[i] = weigh(value_of(s.list[i]));
         __syncthreads();
-        for (int i = tid; i < c; i += NT) {
-          const Entry mine = s.list[i];
-          int count = 0;
-          u64 mass = 0;
-#pragma unroll 4
-          for (int j = 0; j < c; ++j) {
-            const bool front = s.list[j] > mine;
-            count += front;
-            mass += front ? s.lw[j] : 0;
-          }
-          const u64 before = in_front + (by_mass ? mass : (u64)count);
-          if (before < target && target <= before + (by_mass ? s.lw[i] : 1)) {
-            s.chosen_value = value_of(mine);
-            s.chosen_last = column_of(mine);
-            s.chosen_mass = mass + s.lw[i];
-          }
-        }
+        by_teams<NT, u64>(
+            c,
+            [&](int i, int k, int K) {
+              const Entry mine = s.list[i];
+              u64 front = 0;
+#pragma unroll 8
+              for (int j = k; j < c; j += K)
+                front += s.list[j] > mine ? (by_mass ? s.lw[j] : 1) : 0;
+              return front;
+            },
+            [&](int i, u64 front) {
+              const u64 before = in_front + front;
+              if (before < target && target <= before + (by_mass ? s.lw[i] : 1)) {
+                s.chosen_value = value_of(s.list[i]);
+                s.chosen_last = column_of(s.list[i]);
+              }
+            });
         __syncthreads();
         cut = uniform(s.chosen_value);
         last = uniform(s.chosen_last);
-        __syncthreads();
-        return uniform(s.chosen_mass);
+        u64 mass = 0;
+        for (int i = tid; i < c; i += NT) {
+          const float y = value_of(s.list[i]);
+          if (kept(y, column_of(s.list[i]))) mass += s.lw[i];
+        }
+        return block_reduce<NT>(mass, s.redu, AddOp());
       }
       // many entries: halve the bin's range of values
       auto amount = [&](float f) {
@@ -317,7 +350,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
         row.visit([&](int col, float (&x)[4], int) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (x[j] >= f && x[j] > -INFINITY && (x[j] == m ? 0 : bin_of(x[j])) == b &&
+            if (x[j] >= f && x[j] > -INFINITY && bin_of(x[j]) == b &&
                 kept(x[j], col + j))
               q += by_mass ? weigh(x[j]) : 1;
         });
@@ -345,7 +378,7 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
       row.visit([&](int col, float (&x)[4], int) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (x[j] > -INFINITY && (x[j] == m ? 0 : bin_of(x[j])) == b && kept(x[j], col + j) &&
+          if (x[j] > -INFINITY && bin_of(x[j]) == b && kept(x[j], col + j) &&
               (x[j] > f || (x[j] == f && col + j <= c1)))
             mass += weigh(x[j]);
       });
@@ -380,16 +413,26 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
   }
 
   // ---- the draw, in the order of the columns: the weight of each wave's chunks, then the lane
-  auto weight = [&](float x, int col) -> u64 {
-    if (!kept(x, col)) return 0;
-    const double q = weigh.real(x);
-    return q < floor_w ? 0 : weigh.whole(q);
+  const bool cut_off = cut > -INFINITY || last < V - 1, floored = floor_w > 0.0;
+  auto weights = [&](const float (&x)[4], int col, u64 (&q)[4]) {
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      in[j] = !cut_off || kept(clean(x[j]), col + j);
+      q[j] = 0;
+    }
+    if (!__any(in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double f = weigh.real(clean(x[j]));
+      q[j] = in[j] && !(floored && f < floor_w) ? weigh.whole(f) : 0;
+    }
   };
   u64 total = 0;
   row.visit([&](int col, float (&x)[4], int c) {
-    u64 q = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q += weight(clean(x[j]), col + j);
+    u64 four[4];
+    weights(x, col, four);
+    u64 q = four[0] + four[1] + four[2] + four[3];
     if (__any(q != 0)) q = wave_reduce(q, AddOp());
     total += q;
     if (lane == 0) part[c * NW + w] = q;
@@ -416,9 +459,9 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
   if (w == fw)
     row.visit([&](int col, float (&x)[4], int c) {
       if (c != fc) return;
-      u64 q[4], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum += q[j] = weight(clean(x[j]), col + j);
+      u64 q[4];
+      weights(x, col, q);
+      const u64 sum = q[0] + q[1] + q[2] + q[3];
       u64 before = wave_scan(sum) - sum;
       if (rest >= before && rest < before + sum) {
         int pick = 0;

@@ -362,8 +362,7 @@ __device__ __forceinline__ void collect(R& row, Entry* list, int* count, int cap
   __syncthreads();
 }
 
-// How many of the c entries in the list come in front of `mine`.  The list is 16-byte aligned and
-// has an entry to spare.
+// How many of the c entries in the list, which is 16-byte aligned, come in front of `mine`.
 __device__ __forceinline__ int place_of(const Entry* list, int c, Entry mine) {
   struct alignas(16) Two { Entry a, b; };
   const Two* two = reinterpret_cast<const Two*>(list);
@@ -426,7 +425,7 @@ __device__ __forceinline__ float reached_by(R& row, float* gm, float* out, int k
       best = low;
       unsigned lo = key_of(low), hi = key_of(top) + 1;
       int c = kGroups;
-      for (int round = 0; round < 32 && hi - lo > 1 && c > k + k / 4; ++round) {
+      for (int round = 0; round < 32 && hi - lo > 1 && c > k + k / 8; ++round) {
         const unsigned mid = split_key(lo, hi, round);
         const int q = reach(float_of(mid));
         if (q >= k) lo = mid, c = q, best = float_of(mid); else hi = mid;
