@@ -23,18 +23,21 @@ def bucket_probe(on_ready):
     return probe
 
 class BackwardMixin:
-    def train_step(self, x, y, state, on_ready=None, want_extras: bool = False):
+    def train_step(self, x, y, state, on_ready=None, want_extras: bool = False, distill=None):
+        """``distill`` (ops/vocab.py Distill): the loss against a teacher's record, from the
+        logits, in place of the cross-entropy head."""
         B, T = x.shape
         H, V, N, GW = self.H, self.V, T * B, self.GW
-        wide = self._wide_xent(T * B)
+        wide = self._wide_xent(T * B) and distill is None
         # the batch's time-major ids (and the one-hot rows of the embedding-table gradient) are
         # produced by the step's prep launch, not by separate transpose / scatter kernels
         bufs0 = self._buffers(B, T, True)
         ids_tm, tgt = bufs0["ids_tm"], bufs0["tgt_tm"].view(-1)
         id_tasks = self._id_tasks(x, y, bufs0)
         bufs, O, logits, new_state = self._forward(ids_tm, state, True,
-                                                   want_logits=not (self.fused_head
-                                                                    or self.wide_head),
+                                                   want_logits=(distill is not None or not
+                                                                (self.fused_head
+                                                                 or self.wide_head)),
                                                    logits_bias=not wide, extra_tasks=id_tasks)
         # wide vocabulary: the embedding gradient's id sort (three counting-sort launches,
         # csrc/embed.hip id_sort) runs on the side stream beside the (non-persistent) wide head
@@ -85,7 +88,9 @@ class BackwardMixin:
         drop = self._dropout(True)
         dm = self.last_dropout_masks if drop else None
         head_omask = None  # the top output dropout applied by the head kernel to dtop
-        if self.fused_head:
+        if distill is not None:
+            dtop = self._distill_head(distill, O, logits, tgt, bufs, loss_buf, q, tail)
+        elif self.fused_head:
             # one launch: logits (only if asked for) -> CE -> bf16 dlogits, d softmax_b, dtop
             # (masked by the top layer's output dropout in-kernel: no fp32 pass over dtop)
             head_omask = dm["out"] if (dm is not None and self.knobs.on("head_omask")) else None
@@ -563,6 +568,28 @@ class BackwardMixin:
             self._tn_ws = (torch.empty(1024, dtype=f32, device=self.dev),
                            torch.zeros(1, dtype=torch.int32, device=self.dev))
         return self._tn_ws
+
+    def _distill_head(self, d, O, logits, tgt, bufs, loss_buf, q, tail: bool) -> torch.Tensor:
+        """The head of a distillation step: loss and bf16 dlogits in one pass over the logits
+        (csrc/distill.hip), then the head's gradients as on the unfused cross-entropy route."""
+        T, B, k = d.values.shape
+        N, V, s = T * B, self.V, self.store
+        dlog = bufs["dlogits"]
+        self.ops.distill(logits, d.values.reshape(N, k), d.indices.reshape(N, k),
+                         None if d.lse is None else d.lse.reshape(N), tgt, d.alpha,
+                         d.temperature, 1.0 / N, None, bufs["row_loss"], dlog, loss_buf)
+        if bufs["dlogits_pad"] is not None:
+            mm_tn_pad(O, bufs["dlogits_pad"], s.gview("rnnlm/softmax_w"), q=q)
+        else:
+            mm_tn(O, dlog, s.gview("rnnlm/softmax_w"), q=q)
+        gb = s.gview("rnnlm/softmax_b")
+        col = bufs["colsum"][:, :V]
+        self.ops.segsum(dlog, None, 1, col, bufs["ws"], False)
+        gb.copy_(col[0])
+        if tail:
+            q.add_sumsq(gb)
+        dtop = bufs["dtop"].view(N, self.H)
+        return self._dtop_wide(dlog, dtop).view(T, B, self.H)
 
     def _dtop_wide(self, dlog: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
         """dtop = dlogits · softmax_wᵀ (model.py:76's input gradient) for the wide vocabulary:

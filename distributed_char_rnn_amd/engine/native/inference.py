@@ -15,6 +15,15 @@ class InferenceMixin:
         return lg, new_state
 
     @torch.no_grad()
+    def sequence_logits(self, x: torch.Tensor, state):
+        """Every position's logits, time-major [T, B, V] (a buffer that the next call at this
+        shape writes again), and the final state; no dropout."""
+        ids_tm = x.t().contiguous()
+        _, _, logits, new_state = self._forward(ids_tm, state, False)
+        T, B = ids_tm.shape
+        return logits.view(T, B, self.V), new_state
+
+    @torch.no_grad()
     def eval_loss(self, x, y, state):
         ids_tm = x.t().contiguous()
         tgt = y.t().contiguous().view(-1)
@@ -93,6 +102,59 @@ class InferenceMixin:
                 else:
                     one()
         return out.cpu().tolist()
+
+    @torch.no_grad()
+    def sample_filtered(self, prime_ids, num: int, sampling_type: int, u: torch.Tensor,
+                        space_id: int, temperature: float, top_k: int, top_p: float, min_p: float,
+                        use_graph: bool = True):
+        """Sampling under temperature, top-k, top-p and min-p (ops/vocab.py sample_logits) from
+        the uniform numbers ``u`` [num, S]; returns [S][num] ids.  One character is [recurrent
+        step, softmax head, draw], captured once into a hipGraph and replayed; argmax picks
+        (sampling types 0, and 2 where the previous character is no space) are temperature 0."""
+        from ...models.reference import zero_state
+        from ...ops.vocab import sample_logits
+
+        S = u.shape[1]
+        if num <= 0:
+            return [[] for _ in range(S)]
+        state = zero_state(self.cfg, S, self.dev)
+        for cid in prime_ids[:-1]:
+            x = torch.full((S, 1), cid, dtype=torch.int32, device=self.dev)
+            _, state = self.step_logits(x, state)
+        cur = torch.full((S,), int(prime_ids[-1]), dtype=torch.int32, device=self.dev)
+        out = torch.empty(num, S, dtype=torch.int32, device=self.dev)
+        now = torch.empty(S, dtype=torch.float32, device=self.dev)
+        st = [tuple(t.clone() for t in layer) for layer in state]
+        self._run_prep(self._prep())
+
+        def one():
+            _, _, logits, new = self._forward(cur.view(1, S), st, False)
+            t = temperature if sampling_type == 1 else 0.0
+            if sampling_type == 2:
+                t = (cur == space_id).float() * temperature
+            cur.copy_(sample_logits(logits.view(S, self.V), now, t, top_k, top_p, min_p))
+            for a, b in zip(st, new):
+                for x, y in zip(a, b):
+                    x.copy_(y)
+
+        graph = None
+        for i in range(num):
+            now.copy_(u[i])
+            if i == 1 and use_graph and self.knobs.on("sample_graph"):
+                try:
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph):
+                        one()
+                except RuntimeError:
+                    graph = None
+            if graph is not None:
+                graph.replay()
+            else:
+                one()  # (the first character allocates the step's buffers)
+            out[i].copy_(cur)
+        ids = out.t().tolist()
+        self.check_errors()
+        return ids
 
     def _generate_ok(self, S: int) -> bool:
         """The single-launch generator (csrc/generate.hip) covers LSTM stacks of up to 4 layers

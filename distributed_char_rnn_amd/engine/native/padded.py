@@ -114,10 +114,10 @@ class PaddedNativeBackend:
         return [tuple(t[:, : self.H].contiguous() for t in layer) for layer in state]
 
     # -- the backend interface --------------------------------------------------------------
-    def train_step(self, x, y, state, on_ready=None, want_extras: bool = False):
+    def train_step(self, x, y, state, on_ready=None, want_extras: bool = False, distill=None):
         self._sync_params()
         loss, new_state, extras = self.inner.train_step(x, y, self._pad_state(state), None,
-                                                        want_extras=want_extras)
+                                                        want_extras=want_extras, distill=distill)
         self._gather_grads()
         if on_ready is not None:  # padded offsets do not map to the real buckets: all at once
             on_ready(None)
@@ -128,6 +128,11 @@ class PaddedNativeBackend:
         lg, st = self.inner.step_logits(x_t, self._pad_state(state))
         return lg, self._unpad_state(st)
 
+    def sequence_logits(self, x, state):
+        self._sync_params()
+        lg, st = self.inner.sequence_logits(x, self._pad_state(state))
+        return lg, self._unpad_state(st)
+
     def eval_loss(self, x, y, state):
         self._sync_params()
         loss, st = self.inner.eval_loss(x, y, self._pad_state(state))
@@ -136,6 +141,10 @@ class PaddedNativeBackend:
     def sample_sequence(self, *args, **kwargs):
         self._sync_params()
         return self.inner.sample_sequence(*args, **kwargs)
+
+    def sample_filtered(self, *args, **kwargs):
+        self._sync_params()
+        return self.inner.sample_filtered(*args, **kwargs)
 
     def check_errors(self):
         self.inner.check_errors()

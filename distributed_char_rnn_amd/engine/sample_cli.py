@@ -44,7 +44,8 @@ def main(argv=None) -> int:
     model, chars, vocab, _ = load_for_inference(args.save_dir, args.device)
     prime = args.prime or chars[0]  # sample.py:36-37
     outs = sample(model, chars, vocab, args.n, prime, args.sample, seed=args.seed,
-                  num_samples=args.num_samples)
+                  num_samples=args.num_samples, temperature=args.temperature, top_k=args.top_k,
+                  top_p=args.top_p, min_p=args.min_p)
     for o in outs:
         print(o.encode("utf-8") if args.bytes else o)
     return 0

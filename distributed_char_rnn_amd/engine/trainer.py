@@ -34,6 +34,7 @@ from ..utils import checkpoint as ckpt
 from ..utils import data as data_mod
 from ..utils import safe_pickle
 from ..utils.metrics import MetricsLogger, PhaseProfiler, progress_line
+from .distill import Teacher
 from .graph_step import GraphedStep
 from .optim import TFAdam, lr_for_epoch
 
@@ -249,6 +250,12 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
     if start_batch > 0 and saved_state is None:
         _log("warning: the checkpoint holds no TBPTT state for this batch shape (train with "
              "--save_state): the resumed epoch continues from a zero state", rank)
+    teacher = None
+    if getattr(args, "teacher", None):
+        teacher = Teacher.load(args.teacher, loader.chars, device, top_k=args.teacher_top_k,
+                               alpha=args.distill_alpha, temperature=args.distill_temperature)
+        _log(f"distilling from {args.teacher}: top {teacher.k} logits at temperature "
+             f"{teacher.temperature:g}, weight {teacher.alpha:g}", rank)
     ctx.start_heartbeat(getattr(args, "heartbeat", 0.0))
 
     nb = ctx.min_int(loader.num_batches)
@@ -303,6 +310,8 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
         gmode = "off"
     if gmode != "off":
         ok, why = GraphedStep.supported(model, ctx.world_size)
+        if teacher is not None:
+            ok, why = False, "a teacher's forward runs beside every step"
         if ok:
             graphed = GraphedStep(model, opt, log=lambda m: _log(m, rank))
         elif args.graph == "on":
@@ -314,6 +323,8 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
         lr = lr_for_epoch(args.learning_rate, args.decay_rate, e)
         loader.reset_batch_pointer()
         state = model.zero_state(args.batch_size)
+        if teacher is not None:
+            teacher.reset(args.batch_size)
         b0 = start_batch if e == start_epoch else 0
         if b0:
             loader.pointer = b0
@@ -327,10 +338,11 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
             if dev_batches is not None:  # the same batch, already resident on the device
                 x, y = dev_batches[0][b], dev_batches[1][b]
             want = chief and summary_every > 0 and (global_step % summary_every == 0)
+            told = teacher.record(x) if teacher is not None else None
             if zstep is not None:  # sharded optimizer step (ZeRO-1): the backward launches
                 # each bucket's reduce-scatter as soon as its gradients are final
                 with prof.phase("fwd_bwd"):
-                    loss_t, state, extras = _step(model, x, y, state, zstep, want)
+                    loss_t, state, extras = _step(model, x, y, state, zstep, want, told)
                 with prof.phase("sharded_step"):
                     zstep.step(lr)
             elif graphed is not None and not want:
@@ -339,7 +351,7 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
                 extras = None
             else:
                 with prof.phase("fwd_bwd"):
-                    loss_t, state, extras = _step(model, x, y, state, sync, want)
+                    loss_t, state, extras = _step(model, x, y, state, sync, want, told)
                 with prof.phase("grad_sync"):
                     gs = sync.finish(defer_scale=True)
                 with prof.phase("optimizer"):
@@ -371,6 +383,8 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
                     flush(pending, time.time())
                     pending = None
                 model.check_errors()  # never checkpoint weights of a timed-out step
+                if teacher is not None:
+                    teacher.model.check_errors()
                 save_st = None
                 if zstep is not None:
                     zstep.gather_slots()  # collective: the chief saves the full Adam slots
@@ -445,11 +459,12 @@ def _broadcast_state(ctx, model: CharRNN, sd, batch: int, device):
     return out
 
 
-def _step(model: CharRNN, x, y, state, sync, want_extras: bool):
+def _step(model: CharRNN, x, y, state, sync, want_extras: bool, distill=None):
     """``sync``: a GradSync (replicated) or ShardedStep (sharded): both are reset here and
     driven by the backward's readiness callbacks."""
     sync.reset()
-    loss, new_state, extras = model.train_step(x, y, state, sync, want_extras=want_extras)
+    loss, new_state, extras = model.train_step(x, y, state, sync, want_extras=want_extras,
+                                               distill=distill)
     return loss, new_state, (extras if want_extras else None)
 
 

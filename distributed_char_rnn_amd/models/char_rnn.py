@@ -21,6 +21,7 @@ from typing import Optional
 import numpy as np
 import torch
 
+from ..ops.vocab import Distill, top_logits
 from .params import ModelConfig, ParamStore
 from .reference import ReferenceBackend, State, zero_state
 
@@ -84,19 +85,31 @@ class CharRNN:
     def zero_state(self, batch: int) -> State:
         return zero_state(self.cfg, batch, self.device)
 
-    def train_step(self, x, y, state: State, grad_sync=None, want_extras: bool = False):
+    def train_step(self, x, y, state: State, grad_sync=None, want_extras: bool = False,
+                   distill: Optional[Distill] = None):
         """One TBPTT step: forward, loss, backward into ``store.grad``.  ``grad_sync.ready``
-        is called as gradient ranges become final.  Returns (cost tensor, final_state,
-        extras)."""
+        is called as gradient ranges become final.  ``distill`` (:meth:`record_top` of a
+        teacher, with its weight): the loss is the distillation loss against it instead of the
+        cross-entropy.  Returns (cost tensor, final_state, extras)."""
         xi, yi = _as_ids(x, self.device), _as_ids(y, self.device)
         # a disabled sync (one rank) gets no callback: the backend then defers its gradient
         # sums to one launch at the end of the step instead of flushing per bucket
         cb = (grad_sync.ready if grad_sync is not None and getattr(grad_sync, "enabled", True)
               else None)
-        return self.backend.train_step(xi, yi, state, cb, want_extras=want_extras)
+        kw = {} if distill is None else {"distill": distill}
+        return self.backend.train_step(xi, yi, state, cb, want_extras=want_extras, **kw)
 
     def step_logits(self, x_t, state: State):
         return self.backend.step_logits(_as_ids(x_t, self.device), state)
+
+    def record_top(self, x, state: State, k: int, temperature: float = 1.0):
+        """What this model, as a teacher, answers to a batch ``x`` [B, T]: the ``k`` largest logits
+        of every position ``[T, B, k]``, their ids, and the log-sum-exp at ``temperature``
+        ``[T, B]`` (ops/vocab.py top_logits), with the final state."""
+        logits, new_state = self.backend.sequence_logits(_as_ids(x, self.device), state)
+        T, B, V = logits.shape
+        values, indices, lse = top_logits(logits.reshape(T * B, V), k, temperature)
+        return (values.view(T, B, k), indices.view(T, B, k), lse.view(T, B)), new_state
 
     def eval_loss(self, x, y, state: State):
         return self.backend.eval_loss(_as_ids(x, self.device), _as_ids(y, self.device), state)

@@ -29,6 +29,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
+from ..ops.vocab import Distill, distill_loss_rows
 from .params import ModelConfig, ParamStore
 
 State = List[Tuple[torch.Tensor, ...]]
@@ -236,6 +237,20 @@ def loss_fn(logits: torch.Tensor, y: torch.Tensor) -> Tuple[torch.Tensor, torch.
     return per.sum() / per.numel(), per
 
 
+def distill_loss_fn(logits: torch.Tensor, y: torch.Tensor, d: Distill
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`loss_fn` against a teacher's time-major record; ``logits`` are batch-major."""
+    T, B, k = d.values.shape
+
+    def rows(t):
+        return t.transpose(0, 1).reshape((B * T,) + tuple(t.shape[2:])).contiguous()
+
+    return distill_loss_rows(logits, rows(d.values), rows(d.indices),
+                             top_lse=None if d.lse is None else rows(d.lse),
+                             targets=y.reshape(-1).to(torch.int32).contiguous(), alpha=d.alpha,
+                             temperature=d.temperature)
+
+
 class ReferenceBackend:
     """Autograd execution of one TBPTT training step; writes grads into the flat buffer."""
 
@@ -257,13 +272,13 @@ class ReferenceBackend:
         return out
 
     def train_step(self, x, y, state: State, on_bucket_ready=None, want_extras: bool = False,
-                   masks: Optional[dict] = None):
+                   masks: Optional[dict] = None, distill: Optional[Distill] = None):
         params = self.params(True)
         gen = self.gen if self.store.device.type == "cpu" else None
         taps = {}
         logits, new_state, _ = self._forward(self.cfg, params, x, state, training=True, gen=gen,
                                              taps=taps, masks=masks)
-        cost, per = loss_fn(logits, y)
+        cost, per = loss_fn(logits, y) if distill is None else distill_loss_fn(logits, y, distill)
         names = self.store.names()
         grads = torch.autograd.grad(cost, [params[n] for n in names] + [taps["emb"]],
                                     allow_unused=True)
@@ -297,6 +312,14 @@ class ReferenceBackend:
         logits, new_state, _ = self._forward(self.cfg, self.params(False), x_t, state,
                                              training=False)
         return logits, new_state
+
+    @torch.no_grad()
+    def sequence_logits(self, x: torch.Tensor, state: State):
+        """Every position's logits, time-major [T, B, V], and the final state; no dropout."""
+        logits, new_state, _ = self._forward(self.cfg, self.params(False), x, state,
+                                             training=False)
+        B, T = x.shape
+        return logits.view(B, T, -1).transpose(0, 1), new_state
 
     @torch.no_grad()
     def eval_loss(self, x, y, state: State):

@@ -14,7 +14,7 @@ forms at the end.
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -25,6 +25,17 @@ MAX_K = 256     # csrc/kernels.h kRowMaxK: recorded entries a row
 
 Opt = Optional[torch.Tensor]
 Setting = Union[float, torch.Tensor]
+
+
+class Distill(NamedTuple):
+    """What a training step is given of a teacher (``CharRNN.train_step``): its record of the
+    batch, time-major, and how the loss weighs it (see :func:`distill_xent`)."""
+
+    values: torch.Tensor   # [T, B, k] fp32
+    indices: torch.Tensor  # [T, B, k] int32
+    lse: Opt               # [T, B] fp32, at `temperature`
+    alpha: float
+    temperature: float
 
 
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0
@@ -82,6 +93,13 @@ def distill_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
                  top_lse: Opt = None, targets: Opt = None, alpha: float = 1.0,
                  temperature: float = 1.0, scale: Optional[float] = None) -> torch.Tensor:
     """The loss of :func:`distill_xent`, differentiable (once) in ``logits``."""
+    return distill_loss_rows(logits, values, indices, top_lse=top_lse, targets=targets,
+                             alpha=alpha, temperature=temperature, scale=scale)[0]
+
+
+def distill_loss_rows(logits, values, indices, *, top_lse=None, targets=None, alpha=1.0,
+                      temperature=1.0, scale=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`distill_loss` and the row losses (without a gradient of their own)."""
     if scale is None:
         scale = 1.0 / max(1, logits.shape[0])
     return _DistillLoss.apply(logits, values, indices, top_lse, targets, alpha, temperature,
@@ -97,16 +115,18 @@ class _DistillLoss(torch.autograd.Function):
         ctx.save_for_backward(logits, values, indices, lse, targets)
         ctx.args = (alpha, temperature, scale)
         if not logits.is_cuda:
-            return _cpu_distill_xent(logits, values, indices, lse, targets, alpha, temperature,
-                                     scale, None, None)[0]
-        row, loss = _outputs(logits)
-        native.ops().distill(logits, values, indices, lse, targets, alpha, temperature, scale,
-                             None, row, None, loss)
-        return loss
+            loss, row, _ = _cpu_distill_xent(logits, values, indices, lse, targets, alpha,
+                                             temperature, scale, None, None)
+        else:
+            row, loss = _outputs(logits)
+            native.ops().distill(logits, values, indices, lse, targets, alpha, temperature,
+                                 scale, None, row, None, loss)
+        ctx.mark_non_differentiable(row)
+        return loss, row
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
+    def backward(ctx, g, _):
         logits, values, indices, lse, targets = ctx.saved_tensors
         alpha, temperature, scale = ctx.args
         if not logits.is_cuda:

@@ -95,6 +95,17 @@ def train_parser() -> argparse.ArgumentParser:
                    help="emit roctx ranges per phase and print a per-phase timing table")
     g.add_argument("--heartbeat", type=float, default=0.0,
                    help="seconds between rank heartbeats in the rendezvous store (0 = off)")
+    g.add_argument("--teacher", default=None,
+                   help="distil from the trained model in this directory (as --save_dir of its "
+                        "training run): the loss is distill_alpha * T^2 * KL(teacher || student) at "
+                        "temperature T plus (1 - distill_alpha) * cross-entropy")
+    g.add_argument("--teacher_top_k", type=int, default=64,
+                   help="the teacher's largest logits per position that the loss sees (the rest of "
+                        "its probability counts as one); at most 256")
+    g.add_argument("--distill_alpha", type=float, default=0.5,
+                   help="weight of the teacher's answers in the loss, 0 to 1")
+    g.add_argument("--distill_temperature", type=float, default=2.0,
+                   help="temperature at which teacher and student are compared")
     g.add_argument("--graph", default="auto", choices=["auto", "on", "off"],
                    help="replay the whole GPU training step (forward, BPTT, weight gradients, "
                         "clip + Adam) as one captured HIP graph (engine/graph_step.py); auto = "
@@ -113,6 +124,16 @@ def sample_parser() -> argparse.ArgumentParser:
                    help="0 to use max at each timestep, 1 to sample at each timestep, "
                         "2 to sample on spaces")
     p.add_argument("--device", default="auto", choices=["auto", "cpu", "cuda"])
+    p.add_argument("--temperature", type=float, default=1.0,
+                   help="divides the logits before a weighted pick (0: always the largest)")
+    p.add_argument("--top_k", type=int, default=0,
+                   help="weighted picks from the k likeliest characters only (0: all)")
+    p.add_argument("--top_p", type=float, default=1.0,
+                   help="weighted picks from the likeliest characters that make up this share of "
+                        "the probability (1: all)")
+    p.add_argument("--min_p", type=float, default=0.0,
+                   help="weighted picks from characters at least this likely relative to the "
+                        "likeliest (0: all)")
     p.add_argument("--seed", type=int, default=None, help="sampling RNG seed")
     p.add_argument("--num_samples", type=int, default=1,
                    help="independent samples drawn in parallel (batched on the device)")
