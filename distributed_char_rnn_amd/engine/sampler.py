@@ -4,10 +4,11 @@ sample.py:27-46).
 Semantics kept: zero state; feed ``prime[:-1]`` to warm the state; then ``num`` steps from
 ``prime[-1]``; ``sampling_type`` 0 = argmax, 1 = weighted pick (inverse CDF via cumsum +
 searchsorted of ``rand * sum``), 2 = weighted pick only when the *previous* char is a space,
-else argmax.  Beyond the reference, weighted picks can be drawn under a temperature, top-k, top-p
-and min-p (ops/vocab.py ``sample_logits``).  Sampling is batched (``num_samples`` independent streams) and, on the GPU, the
-whole autoregressive loop runs device-side (one fused kernel per generated char, no host sync
-until the end) via the native backend's ``sample_sequence``.
+else argmax.  Beyond the reference, weighted picks can be drawn under a temperature, top-k,
+top-p and min-p (ops/vocab.py ``sample_logits``).  Sampling is batched (``num_samples``
+independent streams) and, on the GPU, the whole autoregressive loop runs device-side (one fused
+kernel per generated char, no host sync until the end) via the native backend's
+``sample_sequence``.
 """
 from __future__ import annotations
 
