@@ -14,38 +14,76 @@
 // that traffic is the bound.  The recorded columns are marked in an LDS bitmap; their threads
 // hold them apart (they write those gradients too), and the rest has a maximum and sum of its
 // own.  So s is never a difference 1 - sum p, which has no digits left where the student is sure.
+//
+// A divergence is a small sum of large terms of both signs.  With sum q + r = sum p + s = 1 it is
+// also the sum of q (d - 1 + exp(-d)), d = log(q / p), over the entries and the rest: no term is
+// negative, none cancels another, and a common error of the log-probabilities drops out.  For the
+// same reason 1 - r / s is taken as sum (q - p) / s where the entries hold little.
 #include "vocab_row.h"
 
 namespace dcr {
+
+namespace {
+
+// d - 1 + exp(-d) = d^2/2! - d^3/3! + ..., up to |d| = 1 (the rest is below 2^-31 of it)
+__device__ __forceinline__ float excess(float d) {
+  float p = 2.0876756987868099e-9f;  // 1 / 12!
+  p = __builtin_fmaf(p, -d, 2.5052108385441719e-8f);
+  p = __builtin_fmaf(p, -d, 2.7557319223985891e-7f);
+  p = __builtin_fmaf(p, -d, 2.7557319223985891e-6f);
+  p = __builtin_fmaf(p, -d, 2.4801587301587302e-5f);
+  p = __builtin_fmaf(p, -d, 1.9841269841269841e-4f);
+  p = __builtin_fmaf(p, -d, 1.3888888888888889e-3f);
+  p = __builtin_fmaf(p, -d, 8.3333333333333333e-3f);
+  p = __builtin_fmaf(p, -d, 4.1666666666666667e-2f);
+  p = __builtin_fmaf(p, -d, 1.6666666666666667e-1f);
+  p = __builtin_fmaf(p, -d, 0.5f);
+  return p * d * d;
+}
+// q d - q + p, for q > 0
+__device__ __forceinline__ float term(float q, float p, float d) {
+  return fabsf(d) <= 1.0f ? q * excess(d) : q * (d - 1.0f) + p;
+}
+
+}  // namespace
 
 template <typename T, typename G, int NT, int EPT>
 __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   constexpr int kE = NT < kRowMaxK ? kRowMaxK / NT : 1;  // entries a thread
   extern __shared__ unsigned bits[];
-  __shared__ float red[(3 + 5 + 2) * (NT / 64)];
+  __shared__ float red[(3 + 5 + 3) * (NT / 64)];
   __shared__ int ei[kRowMaxK], twice;
   __shared__ float eq[kRowMaxK];  // q of the entries, for columns recorded twice
   const long n = blockIdx.x;
   const int tid = threadIdx.x, V = a.r.V, k = a.k;
   const T* z = reinterpret_cast<const T*>(a.r.logits) + n * a.r.ld;
   G* grad = a.grad ? reinterpret_cast<G*>(a.grad) + n * a.grad_ld : nullptr;
-  const float inv_t = 1.0f / a.temperature, c_t = inv_t * 1.44269504088896341f;
+  const float inv_t = a.inv_t, c_t = a.log2e_t;
   constexpr float c_1 = 1.44269504088896341f;
   const int y = a.targets ? a.targets[n] : -1;
   const bool skip = a.targets && (y < 0 || y >= V);
   const bool ce = a.targets && a.alpha < 1.0f;
-  const bool two = ce && inv_t != 1.0f;  // a second exponential an element
+  const bool two = ce && inv_t != 1.0f;
+  // x / T - y with one rounding: 1 / T is a sum of two numbers
+  auto scaled = [&](float x, float y) {
+    return x == -INFINITY ? x : __builtin_fmaf(x, inv_t, __builtin_fmaf(x, a.inv_t_low, -y));
+  };
+  // a second exponential an element
 
-  // ---- the entries: column (-1: none), t / T, the student's z
+  // ---- the entries: column (-1: none), t, the student's z
   int i_e[kE];
   float t_e[kE], z_e[kE];
   bool first[kE];  // the first entry of its column
+  // (k is uniform: a wave passes over the entries that none of it has)
+#define DCR_ENTRIES(e) for (int e = 0; e < kE && (e == 0 || e * NT < k); ++e)
 #pragma unroll
   for (int e = 0; e < kE; ++e) {
     const int j = e * NT + tid;
     i_e[e] = j < k ? a.indices[n * k + j] : -1;
     if (i_e[e] >= V) i_e[e] = -1;
-    t_e[e] = i_e[e] >= 0 ? a.values[n * k + j] * inv_t : -INFINITY;
+    t_e[e] = i_e[e] >= 0 ? a.values[n * k + j] : -INFINITY;
+    z_e[e] = -INFINITY;
+    first[e] = false;
   }
   const float z_y = ce && !skip ? (float)z[y] : 0.f;
   Row<T, NT, EPT> row(z, V);
@@ -53,7 +91,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   if (tid == 0) twice = 0;
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
+  DCR_ENTRIES(e) {
     const int i = i_e[e];
     first[e] = i >= 0;
     z_e[e] = i >= 0 ? (float)z[i] : -INFINITY;
@@ -108,7 +146,7 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   });
   const float mine = top[0];
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
+  DCR_ENTRIES(e) {
     top[1] = fmaxf(top[1], z_e[e]);
     top[2] = fmaxf(top[2], t_e[e]);
   }
@@ -122,12 +160,12 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     sum[1] *= __builtin_amdgcn_exp2f((mine - mr) * c_1);
   }
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
+  DCR_ENTRIES(e) {
     if (first[e] && z_e[e] != -INFINITY) {
-      sum[2] += __expf((z_e[e] - mk) * inv_t);
-      if (two) sum[3] += __expf(z_e[e] - mk);
+      sum[2] += expf(scaled(z_e[e] - mk, 0.f));
+      if (two) sum[3] += expf(z_e[e] - mk);
     }
-    if (t_e[e] != -INFINITY) sum[4] += __expf(t_e[e] - mt);
+    if (t_e[e] != -INFINITY) sum[4] += expf(scaled(t_e[e] - mt, 0.f));
   }
   block_reduce_each<NT, 5>(sum, red + 3 * (NT / 64), AddOp());
   const float sr = sum[0], sr1 = two ? sum[1] : sum[0];
@@ -135,39 +173,59 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
 
   // a skipped row, and one whose mask leaves no column, has neither loss nor gradient
   const bool none = skip || (m == -INFINITY && sr == 0.f && sk == 0.f);
-  // log-sum-exps over m: no logit is scaled by itself, so the lowest values of the type stay finite
+  // sums over m: no logit is scaled by itself, so the lowest values of the type stay finite
   const float dr = mr == -INFINITY ? -INFINITY : mr - m, dk = mk == -INFINITY ? -INFINITY : mk - m;
-  const float lse = __logf(sr * __expf(dr * inv_t) + sk * __expf(dk * inv_t));
-  const float lse1 = __logf(sr1 * __expf(dr) + sk1 * __expf(dk));
+  const float wr = expf(scaled(dr, 0.f)), all = sr * wr + sk * expf(scaled(dk, 0.f));
+  const float lse = logf(all), inv_all = 1.0f / all, off = sr * wr * inv_all;  // off: s
+  const float wr1 = two ? expf(dr) : wr, all1 = two ? sr1 * wr1 + sk1 * expf(dk) : all;
   const bool told = a.lse != nullptr;
   // entries that hold nothing say nothing
-  const float alpha = !told && mt == -INFINITY ? 0.f : a.alpha;
-  const float lt = told ? a.lse[n] : mt + __logf(sum[4]);
-  float q_e[kE], say[2] = {0.f, 0.f};  // sum of q, divergence at the entries
+  const bool mute = !told && mt == -INFINITY;
+  // log q = t / T - lt - log st, where without the teacher's log-sum-exp t counts from its maximum
+  const float lt = told ? a.lse[n] : logf(sum[4]), t0 = told ? 0.f : mt;
+  float q_e[kE], p_e[kE], say[3] = {0.f, 0.f, 0.f};  // sums of q, of the terms, of q - p
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    const float lq = t_e[e] - lt;
-    q_e[e] = t_e[e] != -INFINITY ? __expf(lq) : 0.f;
+  DCR_ENTRIES(e) {
+    const float lq = t_e[e] != -INFINITY ? scaled(t_e[e] - t0, lt) : -INFINITY;
+    const float d = lq - scaled(z_e[e] - m, lse);
+    q_e[e] = expf(lq);
+    p_e[e] = first[e] ? expf(scaled(z_e[e] - m, 0.f)) * inv_all : 0.f;
+    if (i_e[e] < 0 || none) q_e[e] = p_e[e] = 0.f;
     say[0] += q_e[e];
-    if (t_e[e] != -INFINITY && !(q_e[e] <= 0.f)) say[1] += q_e[e] * (lq - ((z_e[e] - m) * inv_t - lse));
+    say[1] += q_e[e] <= 0.f ? p_e[e] : first[e] ? term(q_e[e], p_e[e], d) : q_e[e] * (d - 1.0f);
+    say[2] += q_e[e] - p_e[e];
     if (e * NT + tid < k) eq[e * NT + tid] = q_e[e];
   }
-  block_reduce_each<NT, 2>(say, red + 8 * (NT / 64), AddOp());
+  block_reduce_each<NT, 3>(say, red + 8 * (NT / 64), AddOp());
   if (NT == 64) __syncthreads();  // eq
-  float rest = told ? fmaxf(0.f, 1.0f - say[0]) : 0.f, kl = say[1];
-  if (mr == -INFINITY) rest = 0.f;  // no column to hold it
-  if (rest > 0.f) kl += rest * (__logf(rest) - (dr * inv_t + __logf(sr) - lse));
-  float loss = alpha != 0.f ? alpha * a.temperature * a.temperature * kl : 0.f;
-  if (ce) loss += (1.0f - a.alpha) * (lse1 - (z_y - m));
+  // what the teacher leaves (nothing where no column is left to hold it); the rest's gradient
+  const float rest = told && mr > -INFINITY ? fmaxf(0.f, 1.0f - say[0]) : 0.f;
+  float kl = say[1], pull = wr * inv_all;
+  if (rest > 0.f) {
+    float d;  // log(r / s)
+    if (say[0] < 0.5f && fabsf(say[2]) <= 0.5f * off) {
+      const float gap = say[2] / off;
+      d = log1pf(-gap);
+      pull *= gap;
+    } else {
+      // (s itself may be too small for a number)
+      d = off > 1e-30f ? logf(rest / off) : logf(rest) - (scaled(dr, lse) + logf(sr));
+      pull -= rest / sr;
+    }
+    kl += term(rest, off, d);
+  } else {
+    kl += off + (told ? say[0] - 1.0f : 0.f);
+  }
+  float loss = mute || a.alpha == 0.f ? 0.f : a.alpha_t2 * kl;
+  if (ce) loss += (1.0f - a.alpha) * (logf(all1) - (z_y - m));
   if (tid == 0) a.row_loss[n] = none ? 0.f : loss;
   if (!grad) return;
 
   // ---- the gradient
   const float scale = a.scale * (a.gscale ? *a.gscale : 1.0f);
-  const float ct = alpha * a.temperature * scale, c1 = ce ? (1.0f - a.alpha) * scale : 0.f;
+  const float ct = mute ? 0.f : a.alpha_t * scale, c1 = ce ? (1.0f - a.alpha) * scale : 0.f;
   // weights of exp((z - mr) / T) and exp(z - mr) off the entries
-  float ft = ct * (__expf(dr * inv_t - lse) - (rest > 0.f ? rest / sr : 0.f));
-  float f1 = c1 * __expf(dr - lse1);
+  float ft = ct == 0.f ? 0.f : ct * pull, f1 = c1 * wr1 / all1;
   if (mr == -INFINITY) ft = f1 = 0.f;
   if (!two) ft += f1, f1 = 0.f;
   if (none) ft = f1 = 0.f;
@@ -202,23 +260,26 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
     }
   });
 #pragma unroll
-  for (int e = 0; e < kE; ++e) {
+  DCR_ENTRIES(e) {
     if (!first[e]) continue;
     float q = q_e[e];
     if (twice)
       for (int j = e * NT + tid + 1; j < k; ++j)
         if (ei[j] == i_e[e]) q += eq[j];
-    float g = ct != 0.f ? ct * (__expf((z_e[e] - m) * inv_t - lse) - q) : 0.f;
-    if (ce) g += c1 * __expf(z_e[e] - m - lse1) - (i_e[e] == y ? c1 : 0.f);
+    float g = ct != 0.f ? ct * (p_e[e] - q) : 0.f;
+    if (ce) g += c1 * expf(z_e[e] - m) / all1 - (i_e[e] == y ? c1 : 0.f);
     grad[i_e[e]] = (G)(none ? 0.f : g);
   }
 }
+
+#undef DCR_ENTRIES
 
 // scale * sum of the row losses, in a fixed order
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const float* __restrict__ rows, int n,
                                                            float scale, float* __restrict__ out) {
   __shared__ float red[16];
   float s = 0.f;
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 1024) s += rows[i];
   s = block_reduce<1024>(s, red, AddOp());
   if (threadIdx.x == 0) out[0] = s * scale;
@@ -248,7 +309,14 @@ static void launch_types(const DistillArgs& a, hipStream_t s) {
 #undef CALL
 }
 
-void launch_distill(const DistillArgs& a, hipStream_t s) {
+void launch_distill(const DistillArgs& given, hipStream_t s) {
+  DistillArgs a = given;
+  const double inv = 1.0 / a.temperature;
+  a.inv_t = (float)inv;
+  a.inv_t_low = (float)(inv - (double)a.inv_t);
+  a.log2e_t = (float)(1.4426950408889634 * inv);
+  a.alpha_t = (float)(given.alpha * a.temperature);
+  a.alpha_t2 = (float)(given.alpha * a.temperature * a.temperature);
   if (a.r.N > 0) {
     if (a.r.is_bf16) {
       if (a.grad_bf16) launch_types<bf16, bf16>(a, s); else launch_types<bf16, float>(a, s);

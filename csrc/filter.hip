@@ -195,16 +195,18 @@ __global__ void __launch_bounds__(NT) filter_sample_kernel(FilterArgs a) {
 
   if (want > 0 && want <= kRowMaxK && want < V) {
     // ---- the first `want`, ordered in LDS
-    int c = 0;
-    if constexpr (NT != 64) {
-      const float f = reached_by<NT>(row, s.gm, &s.reached, want);
+    int c = kCap + 1;
+    constexpr int kWaveGroups = EPT >= 16 ? 256 : 0;  // of a row of one wave
+    if (NT != 64 || 4 * want <= kWaveGroups) {
+      const float f = reached_by<NT, NT == 64 ? (kWaveGroups ? kWaveGroups : 64) : kGroups>(
+          row, s.gm, &s.reached, want);
       // (entries of -inf weigh nothing: fewer than `want` others are all that is needed)
       collect<NT>(row, s.list, &s.n, kCap, [&](float x, int) {
         return x >= f && x > -INFINITY;
       });
       c = uniform(s.n);
     }
-    if (NT == 64 || c > kCap) {
+    if (c > kCap) {
       const Cut cut = cut_by_count<NT>(row, s.redi, m, low, want);
       if (tid == 0) s.n = 0;
       __syncthreads();

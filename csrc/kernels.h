@@ -624,7 +624,9 @@ struct DistillArgs {
   const float* values; const int* indices; int k;  // [N, k] recorded entries
   const float* lse;            // optional [N]: the teacher's log-sum-exp (its rest mass counts)
   const int* targets;          // optional [N]
-  float alpha, temperature, scale;
+  float alpha, scale;
+  double temperature;
+  float inv_t, inv_t_low, log2e_t, alpha_t, alpha_t2;  // set by the launcher
   const float* gscale;         // optional device scalar that multiplies the gradient
   float* row_loss;             // [N]
   void* grad; long grad_ld; bool grad_bf16;  // optional [N, V]

@@ -2163,7 +2163,7 @@ void distill(const at::Tensor& logits, const at::Tensor& values, const at::Tenso
     check_rows(*targets, logits, at::kInt, -1, "targets");
     a.targets = ptr<int>(*targets);
   }
-  a.alpha = (float)alpha; a.temperature = (float)temperature; a.scale = (float)scale;
+  a.alpha = (float)alpha; a.temperature = temperature; a.scale = (float)scale;
   if (has(grad_scale)) {
     check_on(*grad_scale, logits, at::kFloat, "grad_scale");
     TORCH_CHECK(grad_scale->numel() == 1, "distill: grad_scale must be one number");
@@ -2186,6 +2186,26 @@ void distill(const at::Tensor& logits, const at::Tensor& values, const at::Tenso
   }
   OnDevice dev(logits);
   dcr::launch_distill(a, dev.stream);
+}
+
+// the same with new tensors: (loss, row losses, gradient in the type of the logits or bf16 / fp32)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> distill_xent(
+    const at::Tensor& logits, const at::Tensor& values, const at::Tensor& indices,
+    const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& targets, double alpha,
+    double temperature, double scale, c10::optional<at::ScalarType> grad_dtype) {
+  check_f32_or_bf16(logits, "logits");
+  TORCH_CHECK(logits.dim() == 2, "distill: logits must be [N, V]");
+  const auto o = logits.options().dtype(at::kFloat);
+  at::Tensor row, loss, grad;
+  {
+    const OnDevice dev(logits);
+    row = at::empty({logits.size(0)}, o);
+    loss = at::empty({}, o);
+    grad = at::empty(logits.sizes(), logits.options().dtype(grad_dtype.value_or(logits.scalar_type())));
+  }
+  distill(logits, values, indices, lse, targets, alpha, temperature, scale, c10::nullopt, row, grad,
+          loss);
+  return {loss, row, grad};
 }
 
 at::Tensor filter_sample(const at::Tensor& logits, const at::Tensor& u, double temperature,
@@ -2455,6 +2475,9 @@ TORCH_LIBRARY(dcr, m) {
   m.def("distill(Tensor logits, Tensor values, Tensor indices, Tensor? lse, Tensor? targets, "
         "float alpha, float temperature, float scale, Tensor? grad_scale, Tensor(a!) row_loss, "
         "Tensor(b!)? grad, Tensor(c!)? loss) -> ()");
+  m.def("distill_xent(Tensor logits, Tensor values, Tensor indices, Tensor? lse, Tensor? targets, "
+        "float alpha, float temperature, float scale, ScalarType? grad_dtype) "
+        "-> (Tensor, Tensor, Tensor)");
   m.def("filter_sample(Tensor logits, Tensor u, float temperature, int top_k, float top_p, "
         "float min_p, Tensor? temperatures=None, Tensor? top_ks=None, Tensor? top_ps=None, "
         "Tensor? min_ps=None) -> Tensor");
@@ -2507,5 +2530,6 @@ TORCH_LIBRARY_IMPL(dcr, CUDA, m) {
   m.impl("linrec_step", &linrec_step);
   m.impl("top_logits", &top_logits);
   m.impl("distill", &distill);
+  m.impl("distill_xent", &distill_xent);
   m.impl("filter_sample", &filter_sample);
 }

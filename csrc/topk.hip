@@ -2,11 +2,11 @@
 // temperature: what a teacher records for distillation.  Order: value descending, ties by the
 // lowest index; NaN counts as -inf in the order and makes the log-sum-exp NaN.
 //
-// One workgroup a row; the row is read once into registers, and that read is the bound.  Up to
-// 1024 columns (one wave) the k-th largest value is found by halving a range of values, with
-// counts by ballot.  Larger rows first find a value that at least k of them reach, from the maxima
-// of 1024 groups of columns; the some k entries that reach it meet in LDS.  Each collected entry
-// finds its place by counting those in front of it.
+// One workgroup a row; the row is read once into registers, and that read is the bound.  From the
+// maxima of groups of columns comes a value that at least k of the row reach; the some k entries
+// that do meet in LDS, and each finds its place by counting those in front of it.  Rows of one wave
+// with k over a quarter of their groups, and rows of many equal values, find the k-th largest
+// value itself by halving a range of values, with counts by ballot.
 #include "vocab_row.h"
 
 namespace dcr {
@@ -22,7 +22,8 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
                                                   float* __restrict__ values,
                                                   int* __restrict__ indices,
                                                   float* __restrict__ lse) {
-  constexpr bool kSmall = NT == 64 && EPT <= 16;
+  constexpr bool kSmall = NT == 64;
+  constexpr int kWaveGroups = EPT >= 16 ? 256 : 0;  // of a row of one wave
   __shared__ float redf[NT / 64];
   __shared__ int redi[NT / 64];
   constexpr int kCap = kSmall ? kRowMaxK : kList;
@@ -61,14 +62,15 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
   }
 
   int c = 0;  // collected entries
-  if constexpr (!kSmall) {
-    const float f = reached_by<NT>(row, gm, &reached, k);
+  if (!kSmall || 4 * k <= kWaveGroups) {
+    const float f = reached_by<NT, kSmall ? (kWaveGroups ? kWaveGroups : 64) : kGroups>(
+        row, gm, &reached, k);
     if (f > -INFINITY) {
-      collect<NT>(row, list, &count, kList, [&](float x, int) { return x >= f; });
+      collect<NT>(row, list, &count, kCap, [&](float x, int) { return x >= f; });
       c = uniform(count);
     }
   }
-  if (c < k || c > kList) {
+  if (c < k || c > kCap) {
     // hardly ever for the long rows: they are read again rather than hold registers for it
     auto again = [&] {
       if constexpr (kSmall) return row;
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
         if (x[j] > -INFINITY) low = fminf(low, x[j]);
     });
     low = block_reduce<NT>(low, redf, MinOp());
-    if (!kSmall && tid == 0) count = 0;
+    if (tid == 0) count = 0;
     const Cut cut = cut_by_count<NT>(again, redi, m, low, k);
     __syncthreads();
     collect<NT>(again, list, &count, k, [&](float x, int col) {

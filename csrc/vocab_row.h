@@ -377,13 +377,13 @@ __device__ __forceinline__ int place_of(const Entry* list, int c, Entry mine) {
 }
 
 // A value that at least k of the row reach and, unless many are equal, few more: the row is cut
-// into kGroups groups of columns, and where k groups have a maximum that high, k values are.
-// With 1024 groups, k <= 256 are a quarter at most and the overshoot stays small.  -inf where
-// fewer than k groups hold anything else.  `gm` holds kGroups values (more than one wave).
-constexpr int kGroups = 1024;
-template <int NT, typename R>
+// into groups of columns, and where k groups have a maximum that high, k values are.  With four
+// times k groups or more the overshoot stays small.  -inf where fewer than k groups hold
+// anything else.  `gm` holds a value a group (more than one wave).
+constexpr int kGroups = 1024;  // for k <= 256
+template <int NT, int GROUPS = kGroups, typename R>
 __device__ __forceinline__ float reached_by(R& row, float* gm, float* out, int k) {
-  constexpr int S = kGroups / NT;  // groups of one thread's chunks
+  constexpr int S = GROUPS / NT;  // groups of one thread's chunks
   float g[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) g[i] = -INFINITY;
@@ -394,7 +394,7 @@ __device__ __forceinline__ float reached_by(R& row, float* gm, float* out, int k
 #pragma unroll
         for (int j = 0; j < 4; ++j) g[i] = fmaxf(g[i], x[j]);
   });
-  constexpr int kPer = kGroups / 64;
+  constexpr int kPer = GROUPS / 64;
   float v[kPer];
   if constexpr (NT == 64) {
 #pragma unroll
@@ -424,7 +424,7 @@ __device__ __forceinline__ float reached_by(R& row, float* gm, float* out, int k
     if (reach(low) >= k) {
       best = low;
       unsigned lo = key_of(low), hi = key_of(top) + 1;
-      int c = kGroups;
+      int c = GROUPS;
       for (int round = 0; round < 32 && hi - lo > 1 && c > k + k / 8; ++round) {
         const unsigned mid = split_key(lo, hi, round);
         const int q = reach(float_of(mid));

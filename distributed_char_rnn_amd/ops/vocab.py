@@ -82,7 +82,8 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
         return _cpu_distill_xent(logits, values, indices, top_lse, targets, alpha, temperature,
                                  scale, grad_dtype, grad)
     if grad is None:
-        grad = torch.empty(logits.shape, dtype=grad_dtype or logits.dtype, device=logits.device)
+        return native.ops().distill_xent(logits, values, indices, top_lse, targets, alpha,
+                                         temperature, scale, grad_dtype)
     row, loss = _outputs(logits)
     native.ops().distill(logits, values, indices, top_lse, targets, alpha, temperature, scale,
                          None, row, grad, loss)
@@ -234,8 +235,8 @@ def _cpu_distill_xent(logits, values, indices, lse, targets, alpha, tau, scale, 
         out = torch.logsumexp(torch.where(entry, -math.inf, logp), 1)
         left = (rest > 0) & ~torch.isneginf(out)
         kl = kl + torch.where(left, rest * (rest.log() - out), 0.0)
-        share = torch.where(left, (rest.log() - out).exp(), 0.0)
-        g = torch.where(entry, g, g * (1.0 - share[:, None]))
+        gone = torch.where(left, rest.log() - out, -math.inf)[:, None]
+        g = torch.where(entry, g, g - torch.where(left[:, None], (logp + gone).exp(), 0.0))
     else:
         on = some.float()[:, None]
         kl = torch.where(some, kl, 0.0)

@@ -263,6 +263,47 @@ def test_distill_lowest_values(tau, dtype, dev):
     assert ((grad.double().cpu() - gwant).abs() <= tol + half * (gwant.abs() + tol)).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V,k,tau", [(12, 2136, 1, 3.278), (306, 1909, 63, 2.844),
+                                       (8, 151, 77, 0.929), (4, 9000, 4, 5.0), (4, 70000, 2, 4.0)])
+def test_distill_small_divergences_keep_their_digits(N, V, k, tau):
+    """A student near its teacher, few recorded tokens: the divergence is some 1e-3 of its terms.
+    It is a sum of q (d - 1 + exp(-d)), d = log(q / p), none negative and each with a relative error
+    of 2 err(d) / |d|; the weighted |d| is sqrt(2 KL), err(d) under 32 u.  The gradient's error is that
+    of p and q, 128 u of p each (q < 2 p).  Off the entries it is T p (1 - r / s) with r = 1 - sum q: where
+    the entries hold most, r has the absolute error of that sum, 32 u of sum q <= 1 and k u from
+    adding, and the gradient p / s of it; where they hold little, 1 - r / s = sum (q - p) / s has
+    64 u of sum (q + p) <= 1.5, over s > 1/4."""
+    z = rows(N, V, F32, "cuda")
+    g = torch.Generator().manual_seed(5)
+    t = z.cpu() + 0.1 * torch.randn(z.shape, generator=g)
+    top = torch.topk(t, k, dim=1)
+    values, indices = top.values.cuda(), top.indices.int().cuda()
+    lse = torch.logsumexp(t.double() / tau, 1).float().cuda()
+    _, row, grad = O.distill_xent(z, values, indices, top_lse=lse, temperature=tau)
+    want, gwant = reference_distill(z, values, indices, lse, None, 1.0, tau, 1.0 / N)
+    kl = want / tau ** 2
+    assert (kl < 0.05).all()
+    err = (row.double().cpu() - want).abs() / tau ** 2
+    assert (err <= 64 * U * (2 * kl).sqrt() + 64 * U * kl).all(), (err / kl).max()
+    p = torch.softmax(z.double().cpu() / tau, 1)
+    off = torch.ones_like(p).scatter(1, indices.long().cpu(), 0.0)
+    s = (p * off).sum(1, keepdim=True)
+    allowed = 256 * U * p + off * p / s * (k + 96) * U
+    assert ((grad.double().cpu() - gwant).abs() <= allowed * tau / N + 1e-12).all()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_distill_sure_students(dev):
+    """The student's mass off the entries is too small for fp32: the divergence is still a number."""
+    V = 500
+    z = torch.full((2, V), -60.0, device=dev)
+    z[:, 3:5] = 60.0
+    values = torch.tensor([[2.0, 1.0], [-3.0, -3.5]], device=dev)
+    indices = torch.tensor([[3, 4]] * 2, dtype=torch.int32, device=dev)
+    check_distill(z, values, indices, torch.tensor([2.6, 2.0], device=dev), None, 1.0, 1.0)
+
+
 @pytest.mark.parametrize("dev", DEVS)
 def test_distill_infinite_and_nan(dev):
     z = rows(4, 70, F32, dev)
