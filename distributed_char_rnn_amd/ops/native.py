@@ -77,3 +77,15 @@ def ops():
     if not try_load(build_if_missing=os.environ.get("DCR_AUTOBUILD", "1") == "1"):
         raise RuntimeError(_err or "native library unavailable")
     return torch.ops.dcr
+
+
+_resolved: dict = {}
+
+
+def op(name: str):
+    """The one overload of ``torch.ops.dcr.<name>``, looked up once: for calls that are as short
+    as their launch (a lookup through :func:`ops` and overload resolution cost some 2 us)."""
+    f = _resolved.get(name)
+    if f is None:
+        f = _resolved[name] = getattr(ops(), name).default
+    return f

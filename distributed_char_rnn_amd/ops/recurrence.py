@@ -34,7 +34,7 @@ def linear_recurrence_fwd(x: torch.Tensor, f: torch.Tensor, h0: Opt = None, *,
     """``(h [T, B, H], final state [B, H], carry)``.  ``carry`` holds the fp32 states that
     :func:`linear_recurrence_bwd` starts from; it is empty without ``want_carry``."""
     if x.is_cuda:
-        return native.ops().linrec_fwd(x, f, h0, lengths, starts, want_carry)
+        return native.op("linrec_fwd")(x, f, h0, lengths, starts, want_carry)
     _check(x, f, h0, lengths, starts)
     return _cpu_fwd(x, f, h0, lengths, starts, want_carry)
 
@@ -47,7 +47,7 @@ def linear_recurrence_bwd(x: torch.Tensor, f: torch.Tensor, carry: torch.Tensor,
     final state (``dlast`` fp32, absent: zero).  ``x``, ``f``, ``lengths`` and ``starts`` are the
     forward's, ``carry`` what it returned."""
     if x.is_cuda:
-        return native.ops().linrec_bwd(x, f, carry, dh, dlast, lengths, starts)
+        return native.op("linrec_bwd")(x, f, carry, dh, dlast, lengths, starts)
     _check(x, f, dlast, lengths, starts)
     torch._check(dh.shape == x.shape and dh.dtype == x.dtype, lambda: "dh must be like x")
     torch._check(carry.shape == x.shape, lambda: "carry must be the forward's")
@@ -59,7 +59,7 @@ def linear_recurrence_step(x: torch.Tensor, f: torch.Tensor, h: torch.Tensor, *,
     """One step of every stream: ``x``, ``f`` ``[B, H]``; the fp32 state ``h`` is updated in
     place and its copy in ``x``'s type returned.  ``starts``: bool ``[B]``."""
     if x.is_cuda:
-        return native.ops().linrec_step(x, f, h, starts)
+        return native.op("linrec_step")(x, f, h, starts)
     torch._check(x.dim() == 2, lambda: "x and f must be [B, H]")
     torch._check(h.is_contiguous(), lambda: "h must be contiguous")
     st = None if starts is None else starts[None]

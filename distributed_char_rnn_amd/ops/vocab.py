@@ -45,7 +45,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0
     ``log sum exp(logits / temperature)`` over the whole row.  NaN counts as -inf in the order
     and makes the row's ``lse`` NaN."""
     if logits.is_cuda:
-        return native.ops().top_logits(logits, k, temperature)
+        return native.op("top_logits")(logits, k, temperature)
     _check_logits(logits)
     torch._check(1 <= k <= min(MAX_K, logits.shape[1]), lambda: f"k must be 1 to {MAX_K} and V")
     _check_temperature(temperature)
@@ -82,10 +82,10 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
         return _cpu_distill_xent(logits, values, indices, top_lse, targets, alpha, temperature,
                                  scale, grad_dtype, grad)
     if grad is None:
-        return native.ops().distill_xent(logits, values, indices, top_lse, targets, alpha,
+        return native.op("distill_xent")(logits, values, indices, top_lse, targets, alpha,
                                          temperature, scale, grad_dtype)
     row, loss = _outputs(logits)
-    native.ops().distill(logits, values, indices, top_lse, targets, alpha, temperature, scale,
+    native.op("distill")(logits, values, indices, top_lse, targets, alpha, temperature, scale,
                          None, row, grad, loss)
     return loss, row, grad
 
@@ -120,7 +120,7 @@ class _DistillLoss(torch.autograd.Function):
                                              temperature, scale, None, None)
         else:
             row, loss = _outputs(logits)
-            native.ops().distill(logits, values, indices, lse, targets, alpha, temperature,
+            native.op("distill")(logits, values, indices, lse, targets, alpha, temperature,
                                  scale, None, row, None, loss)
         ctx.mark_non_differentiable(row)
         return loss, row
@@ -137,7 +137,7 @@ class _DistillLoss(torch.autograd.Function):
         else:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             row = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-            native.ops().distill(logits, values, indices, lse, targets, alpha, temperature, scale,
+            native.op("distill")(logits, values, indices, lse, targets, alpha, temperature, scale,
                                  g, row, grad, None)
         return (grad,) + (None,) * 7
 
@@ -165,7 +165,7 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     k, ks = _setting(top_k, 0)
     p, ps = _setting(top_p, 1.0)
     q, qs = _setting(min_p, 0.0)
-    return native.ops().filter_sample(logits, u, t, k, p, q, ts, ks, ps, qs)
+    return native.op("filter_sample")(logits, u, t, k, p, q, ts, ks, ps, qs)
 
 
 def _setting(v, default):
