@@ -1979,8 +1979,9 @@ dcr::LinrecArgs linrec_args(const at::Tensor& x, const at::Tensor& f,
   TORCH_CHECK(x.dim() == 3, op, ": x must be [T, B, H]");
   check_seq3(x, x, "x");
   check_seq3(f, x, "f");
-  TORCH_CHECK(x.size(0) < (1 << 30) && x.size(1) < (1 << 30) && x.size(2) < (1 << 30) &&
-                  x.size(1) * x.size(2) < (1LL << 31), op, ": sizes too large");
+  // (a launch holds fewer than 2^32 threads, eight a channel at most)
+  TORCH_CHECK(x.size(0) < (1 << 30) && x.size(1) <= (1 << 28) && x.size(2) <= (1 << 28) &&
+                  x.size(1) * x.size(2) <= (1LL << 28), op, ": at most 2^30 steps and 2^28 channels");
   dcr::LinrecArgs a{};
   a.T = (int)x.size(0); a.B = (int)x.size(1); a.H = (int)x.size(2);
   a.x = x.data_ptr(); a.x_t = x.stride(0); a.x_b = x.stride(1);
@@ -2099,7 +2100,7 @@ dcr::RowArgs row_args(const at::Tensor& logits, const char* op) {
   const int64_t N = logits.size(0), V = logits.size(1);
   TORCH_CHECK(V >= 1 && V <= dcr::kRowMaxV, op, ": vocabularies of 1 to ", dcr::kRowMaxV,
               " entries, got ", V);
-  TORCH_CHECK(N < (1LL << 31), op, ": too many rows");
+  TORCH_CHECK(N < (1LL << 22), op, ": fewer than 2^22 rows, got ", N);  // 2^32 threads a launch
   TORCH_CHECK(V == 1 || logits.stride(1) == 1, op, ": logits need unit stride along the vocabulary");
   dcr::RowArgs r{};
   r.logits = logits.data_ptr(); r.ld = logits.stride(0); r.N = (int)N; r.V = (int)V;

@@ -129,7 +129,7 @@ class InferenceMixin:
 
         def one():
             _, _, logits, new = self._forward(cur.view(1, S), st, False)
-            t = temperature if sampling_type == 1 else 0.0
+            t = 0.0 if sampling_type == 0 else temperature
             if sampling_type == 2:
                 t = (cur == space_id).float() * temperature
             cur.copy_(sample_logits(logits.view(S, self.V), now, t, top_k, top_p, min_p))

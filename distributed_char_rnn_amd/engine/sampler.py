@@ -101,7 +101,7 @@ def _sample_filtered(model: CharRNN, prime: Sequence[int], num: int, sampling_ty
         cur.fill_(prime[-1])
         for i in range(num):
             logits, state = model.step_logits(cur[:, None], state)
-            t = temperature if sampling_type == 1 else 0.0
+            t = 0.0 if sampling_type == 0 else temperature
             if sampling_type == 2:
                 t = (cur == space_id).float() * temperature
             cur = sample_logits(logits, u[i], t, top_k, top_p, min_p)

@@ -327,6 +327,8 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
             teacher.reset(args.batch_size)
         b0 = start_batch if e == start_epoch else 0
         if b0:
+            for i in range(b0 if teacher is not None else 0):  # the teacher's state in front of b0
+                teacher.record(loader.x_batches[i] if dev_batches is None else dev_batches[0][i])
             loader.pointer = b0
             if saved_state is not None:  # the carry of the interrupted run's batch b0 - 1
                 state = saved_state

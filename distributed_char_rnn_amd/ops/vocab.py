@@ -1,5 +1,6 @@
 """Operators over rows of vocabulary logits ``[N, V]`` (fp32 or bf16, unit stride along the
-vocabulary, any row stride, V up to 262144), beside the cross-entropy and the sampling step:
+vocabulary, any row stride, V up to 262144, on the GPU fewer than 2^22 rows), beside the
+cross-entropy and the sampling step:
 
 * :func:`top_logits` -- what a teacher records of its answer: the k largest logits of a row and
   the log-sum-exp at a temperature;

@@ -147,6 +147,39 @@ def test_teacher_refuses():
             Teacher(t, **kw)
 
 
+@pytest.mark.parametrize("dev", DEVS)
+def test_resume_gives_the_teacher_its_state_back(tmp_path, dev, monkeypatch):
+    """A run resumed in the middle of an epoch sees the records of the uninterrupted run."""
+    from distributed_char_rnn_amd.engine import trainer
+    from distributed_char_rnn_amd.utils.config import train_parser
+
+    monkeypatch.chdir(tmp_path)
+    common = ["--synthetic_text", "2000", "--batch_size", "4", "--seq_length", "20", "--num_epochs",
+              "1", "--log_dir", "logs", "--summary_every", "0", "--device", dev, "--rnn_size", "32"]
+    seen = []
+    record = Teacher.record
+
+    def spy(self, x):
+        d = record(self, x)
+        seen.append(d.values.float().cpu())
+        return d
+
+    def run(*args):
+        seen.clear()
+        assert trainer.train(train_parser().parse_args(common + list(args))) == 0
+        return list(seen)
+
+    run("--save_dir", "t", "--max_steps", "3")
+    monkeypatch.setattr(Teacher, "record", spy)
+    whole = run("--save_dir", "a", "--teacher", "t", "--max_steps", "6")
+    run("--save_dir", "b", "--teacher", "t", "--max_steps", "3", "--save_state")
+    rest = run("--save_dir", "c", "--teacher", "t", "--init_from", "b", "--resume_exact",
+               "--max_steps", "3")
+    assert len(whole) == 6 and len(rest) == 6  # three to catch up, three of its own
+    for a, b in zip(whole, rest):
+        assert torch.equal(a, b)
+
+
 # ---- sampling ---------------------------------------------------------------------------------
 CHARS = [" "] + [chr(97 + i) for i in range(25)]
 

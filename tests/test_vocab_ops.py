@@ -563,6 +563,18 @@ def test_refusals(dev):
 
 
 @pytest.mark.gpu
+def test_refuses_more_rows_than_a_launch_holds():
+    z = torch.zeros(1, 3, device="cuda").expand(1 << 22, 3)
+    with pytest.raises(RuntimeError):
+        O.top_logits(z, 2)
+    with pytest.raises(RuntimeError):
+        O.sample_logits(z, torch.zeros(1 << 22, device="cuda"))
+    x = torch.zeros(1, 1, 1, device="cuda").expand(2, 1 << 15, (1 << 13) + 1)
+    with pytest.raises(RuntimeError):
+        torch.ops.dcr.linrec_fwd(x, x, None, None, None, False)
+
+
+@pytest.mark.gpu
 def test_refuses_mixed_devices():
     z = rows(4, 65, F32, "cuda")
     v, i, lse = O.top_logits(z, 4)
