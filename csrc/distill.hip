@@ -288,9 +288,12 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const float* __restri
 // Workgroup and registers for N rows of V columns.  One wave takes a row of up to 1024 columns: no
 // barriers, and many rows a CU.  Up to 16384 columns, few rows get more threads, which is faster for
 // the row, and many get smaller workgroups, whose loads and computations overlap each other's
-// (fp32: 256 x 8192 7.8 us with 512 threads, 14.8 with 128; 32768 x 8192 343 with 128, 374 with 256).
-// Past 32768 the registers are too few for two workgroups a CU, and a row is read twice instead
-// (1024 x 65536 bf16: 101 us, 115 from registers).
+// (fp32 to bf16, two exponentials: 256 x 8192 8.3 us with 512 threads, 15.6 with 128; 32768 x 8192 359
+// with 128, 401 with 256; 5296 x 12157 bf16 85 with 256, 102 with 512).  Past 32768 the registers are
+// too few for two workgroups a CU, and a row is read twice instead (1024 x 65536 bf16: 106 us, 121 from
+// registers).  Against the traffic at the rate of a large copy (5.0 TB/s): 32768 x 8192 318 us, 5296 x
+// 12157 51, 2047 x 32001 52 (89 measured: conversions and exponentials of both passes take their
+// share of issue slots beside two workgroups' loads).
 template <typename T, typename G>
 static void launch_types(const DistillArgs& a, hipStream_t s) {
   const size_t lds = (size_t)((a.r.V + 31) / 32) * 4;

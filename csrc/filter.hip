@@ -18,6 +18,10 @@
 //                     interval that holds a border; its entries meet in LDS, are ordered, and the
 //                     border is the one entry in front of which less than the target lies.
 //   otherwise         nothing to find: min_p is a bound on the value.
+// 256 rows of 32001 bf16: all kept 20 us, top_k 50 16, top_p 42, every row with settings of its own
+// 46: the 64-bit exponential of every token and, for top_p, an LDS addition each are what bounds it
+// (the read alone is 3 us).  16 rows of 65: 7.3 us with the launch.
+//
 // An interval that holds more than kList entries (rows of many equal values) is halved by values
 // until one value is left, as a whole: slow, and hardly ever.
 #include "vocab_row.h"

@@ -7,6 +7,10 @@
 // that do meet in LDS, and each finds its place by counting those in front of it.  Rows of one wave
 // with k over a quarter of their groups, and rows of many equal values, find the k-th largest
 // value itself by halving a range of values, with counts by ballot.
+//
+// 32768 x 8192 fp32, k = 64: 241 us, 4.5 TB/s (a large copy reaches 5.0); k = 200 398 us, where the
+// places of some 220 entries are the work.  10222 x 864 bf16, k = 31: 20 us; with k = 131, past a
+// quarter of the groups, 78.
 #include "vocab_row.h"
 
 namespace dcr {
