@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const float* __restri
 // barriers, and many rows a CU.  Up to 16384 columns, few rows get more threads, which is faster for
 // the row, and many get smaller workgroups, whose loads and computations overlap each other's
 // (fp32 to bf16, two exponentials: 256 x 8192 8.3 us with 512 threads, 15.6 with 128; 32768 x 8192 359
-// with 128, 401 with 256; 5296 x 12157 bf16 85 with 256, 102 with 512).  Past 32768 the registers are
+// with 128, 401 with 256; 5296 x 12157 bf16 85 with 256, 102 with 512; 21294 x 1897 bf16 80 with 64, 120
+// with 256).  Past 32768 the registers are
 // too few for two workgroups a CU, and a row is read twice instead (1024 x 65536 bf16: 106 us, 121 from
 // registers).  Against the traffic at the rate of a large copy (5.0 TB/s): 32768 x 8192 318 us, 5296 x
 // 12157 51, 2047 x 32001 52 (89 measured: conversions and exponentials of both passes take their
@@ -302,6 +303,8 @@ static void launch_types(const DistillArgs& a, hipStream_t s) {
 #define CALL(NTH, E) distill_kernel<T, G, NTH, E><<<a.r.N, NTH, lds, s>>>(a)
   if (V <= 256) CALL(64, 4);
   else if (V <= 1024) CALL(64, 16);
+  else if (V <= 2048 && many) CALL(64, 32);
+  else if (V <= 4096 && many) CALL(128, 32);
   else if (V <= 4096) CALL(256, 16);
   else if (V <= 8192 && many) CALL(128, 64);
   else if (V <= 8192) CALL(512, 16);

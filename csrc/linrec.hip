@@ -88,6 +88,29 @@ struct Lane {  // one lane's VEC channels
   int h;
 };
 
+// v through the pairs of n segments from `first` on, a batch of loads at a time (one after the other
+// they would cost a cache's latency each).
+template <bool MARKS, int VEC>
+__device__ __forceinline__ void fold_pairs(float (&v)[VEC], const LinrecArgs& p, long c, int first,
+                                           int dir, int n) {
+  constexpr int kBatch = 16 / VEC;
+  const long BH = (long)p.B * p.H;
+  for (int s = 0; s < n; s += kBatch) {
+    float A[kBatch][VEC], B[kBatch][VEC];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const long at = (first + dir * min(s + i, n - 1)) * BH + c;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) A[i][j] = p.sumA[at + j], B[i][j] = p.sumB[at + j];
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (s + i < n)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = step_<MARKS>(A[i][j], v[j], B[i][j]);
+  }
+}
+
 // The second launch takes the segments the other way round: what the first read last is still
 // in the last-level cache.
 template <bool SUMMARY>
@@ -131,12 +154,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
     carry[j] = (!SUMMARY && p.h0) ? p.h0[l.c + j] : 0.f;
     pa[j] = 1.f;
   }
-  if (!SUMMARY)
-#pragma unroll 4
-    for (int s = 0; s < seg; ++s)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        carry[j] = step_<MARKS>(p.sumA[s * BH + l.c + j], carry[j], p.sumB[s * BH + l.c + j]);
+  if (!SUMMARY) fold_pairs<MARKS, VEC>(carry, p, l.c, 0, 1, seg);
 
   const int tile1 = min((seg + 1) * p.tiles_per_seg, p.tiles);
   int buf = 0;
@@ -236,11 +254,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
     pa[j] = 1.f;
   }
   if (!SUMMARY)
-#pragma unroll 4
-    for (int s = (int)gridDim.y - 1; s > seg; --s)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        e[j] = step_<MARKS>(p.sumA[s * BH + l.c + j], e[j], p.sumB[s * BH + l.c + j]);
+    fold_pairs<MARKS, VEC>(e, p, l.c, (int)gridDim.y - 1, -1, (int)gridDim.y - 1 - seg);
 
   const int tile1 = min((seg + 1) * p.tiles_per_seg, p.tiles);
   int buf = 0;
