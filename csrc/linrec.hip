@@ -426,20 +426,22 @@ void run_type(LinrecArgs& p, bool bwd, int vec, hipStream_t s) {
 //  * segments where even single channels leave fewer workgroups and there are 512 steps or more,
 //    although x, f and dh are then read twice (4096 steps of 512 channels: 12.6 / 18.3 with 64
 //    segments, 41 / 56 with 16); for 200 steps of 6400 channels one segment takes 8.7 / 12.0, eight
-//    11.0 / 12.8.  At most 64: each workgroup folds the pairs in front of its segment.
+//    11.0 / 12.8.  At most 128 (15390 steps of 384 channels
+//    bf16, forward and backward: 68 us, with at most 64 78): each workgroup folds the pairs in
+//    front of its segment.
 LinrecPlan linrec_plan(int T, int B, int H) {
   LinrecPlan q{};
   auto wgs = [&](int vec) { return ((long)B * (H / vec) + 63) / 64; };
   const int widest = H % 4 == 0 ? 4 : H % 2 == 0 ? 2 : 1;
   const bool split = T >= 512 && wgs(1) < 192;
-  const long cuts = split ? (T / 64 < 64 ? T / 64 : 64) : 1;
+  const long cuts = split ? (T / 64 < 128 ? T / 64 : 128) : 1;
   q.vec = widest;
   while (q.vec > 1 && wgs(q.vec) * cuts < (split ? 512 : 192)) q.vec /= 2;
   const long n = wgs(q.vec) > 0 ? wgs(q.vec) : 1;
   q.waves = T <= 32 || q.vec == 4 ? 4 : 8;
   q.tiles = (T + q.waves * kC - 1) / (q.waves * kC);
   long segs = split ? ((q.waves == 4 ? 1024 : 512) + n - 1) / n : 1;
-  if (segs > 64) segs = 64;
+  if (segs > 128) segs = 128;
   q.tiles_per_seg = (int)((q.tiles + segs - 1) / segs);
   if (q.tiles_per_seg < 1) q.tiles_per_seg = 1;
   q.segs = (q.tiles + q.tiles_per_seg - 1) / q.tiles_per_seg;
