@@ -404,7 +404,7 @@ void run_type(LinrecArgs& p, bool bwd, int vec, hipStream_t s) {
   const bool marks = p.lengths || p.starts;
 #define LR(VV) \
   if (marks) run_seq<T, VV, W, true>(p, bwd, s); else run_seq<T, VV, W, false>(p, bwd, s)
-  if constexpr (W == 4) {
+  if constexpr (W <= 4) {
     if (vec == 4) {
       LR(4);
       return;
@@ -420,15 +420,15 @@ void run_type(LinrecArgs& p, bool bwd, int vec, hipStream_t s) {
 // backward has to find the forward's tiles).  Measured on one MI355X, forward / backward us:
 //  * the widest loads that leave some 192 workgroups, else single channels: 25600 channels, 1024
 //    steps, bf16: 51 / 68 with two channels a lane, 52 / 78 with one, 108 / 135 with four;
-//  * four waves where a lane has four channels (128 steps of 256 x 512 bf16: 25 / 37, with eight
-//    25 / 42; 16384 steps of 4 x 1000, padded documents: 165 / 232 against 184 / 275), else eight:
-//    longer tiles, fewer of them (4096 steps of 512 channels: 12.6 / 18.3, with four 14.5 / 21.0);
+//  * no more waves than the steps fill (8 steps of 256 x 2048 bf16, both directions: 19 with one, 41
+//    with four); then four waves where a lane has four channels (128 steps of 256 x 512 bf16: 25 / 37,
+//    with eight 25 / 42; 16384 steps of 4 x 1000, padded documents: 165 / 232 against 184 / 275), else
+//    eight: longer tiles, fewer of them (4096 steps of 512 channels: 12.6 / 18.3, with four 14.5 / 21.0);
 //  * segments where even single channels leave fewer workgroups and there are 512 steps or more,
 //    although x, f and dh are then read twice (4096 steps of 512 channels: 12.6 / 18.3 with 64
 //    segments, 41 / 56 with 16); for 200 steps of 6400 channels one segment takes 8.7 / 12.0, eight
-//    11.0 / 12.8.  At most 128 (15390 steps of 384 channels
-//    bf16, forward and backward: 68 us, with at most 64 78): each workgroup folds the pairs in
-//    front of its segment.
+//    11.0 / 12.8.  At most 128 (15390 steps of 384 channels bf16, both directions: 68, with at most
+//    64 78): each workgroup folds the pairs in front of its segment.
 LinrecPlan linrec_plan(int T, int B, int H) {
   LinrecPlan q{};
   auto wgs = [&](int vec) { return ((long)B * (H / vec) + 63) / 64; };
@@ -438,7 +438,7 @@ LinrecPlan linrec_plan(int T, int B, int H) {
   q.vec = widest;
   while (q.vec > 1 && wgs(q.vec) * cuts < (split ? 512 : 192)) q.vec /= 2;
   const long n = wgs(q.vec) > 0 ? wgs(q.vec) : 1;
-  q.waves = T <= 32 || q.vec == 4 ? 4 : 8;
+  q.waves = T <= kC ? 1 : T <= 2 * kC ? 2 : T <= 4 * kC || q.vec == 4 ? 4 : 8;
   q.tiles = (T + q.waves * kC - 1) / (q.waves * kC);
   long segs = split ? ((q.waves == 4 ? 1024 : 512) + n - 1) / n : 1;
   if (segs > 128) segs = 128;
@@ -454,11 +454,11 @@ void launch_linrec(LinrecArgs p, bool is_bf16, bool bwd, hipStream_t s) {
   p.tiles = q.tiles;
   p.tiles_per_seg = q.tiles_per_seg;
   p.segs = q.segs;
-  if (is_bf16) {
-    if (q.waves == 4) run_type<bf16, 4>(p, bwd, q.vec, s); else run_type<bf16, 8>(p, bwd, q.vec, s);
-  } else {
-    if (q.waves == 4) run_type<float, 4>(p, bwd, q.vec, s); else run_type<float, 8>(p, bwd, q.vec, s);
-  }
+#define LW(WW) \
+  if (is_bf16) run_type<bf16, WW>(p, bwd, q.vec, s); else run_type<float, WW>(p, bwd, q.vec, s)
+  if (q.waves == 1) { LW(1); } else if (q.waves == 2) { LW(2); }
+  else if (q.waves == 4) { LW(4); } else { LW(8); }
+#undef LW
 }
 
 void launch_linrec_step(const LinrecArgs& p, bool is_bf16, hipStream_t s) {
