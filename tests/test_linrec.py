@@ -267,6 +267,35 @@ def test_autograd_matches_explicit_and_differences(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+def test_lengths_are_clamped(dev):
+    args = inputs(23, 4, 10, F32, dev)
+    odd = torch.tensor([-5, 99, 23, 7], dtype=torch.int32, device=dev)
+    a = R.linear_recurrence_fwd(*args[:3], lengths=odd)
+    b = R.linear_recurrence_fwd(*args[:3], lengths=odd.clamp(0, 23))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    g = [R.linear_recurrence_bwd(*args[:2], a[2], args[3], dlast=args[4], lengths=n)
+         for n in (odd, odd.clamp(0, 23))]
+    assert all(torch.equal(p, q) for p, q in zip(*g))
+
+
+@pytest.mark.gpu
+def test_far_offsets():
+    """Steps more than 2^31 elements apart."""
+    T, B, H, far = 3, 2, 64, (1 << 30) + 64
+    small = inputs(T, B, H, BF16, "cuda")
+    bufs = [torch.empty(2 * far + B * H, dtype=BF16, device="cuda") for _ in range(3)]
+    x, f, dh = (torch.as_strided(b, (T, B, H), (far, H, 1)) for b in bufs)
+    for v, s in zip((x, f, dh), (small[0], small[1], small[3])):
+        v.copy_(s)
+    a = R.linear_recurrence_fwd(x, f, small[2])
+    b = R.linear_recurrence_fwd(*small[:3])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    g = R.linear_recurrence_bwd(x, f, a[2], dh, dlast=small[4])
+    w = R.linear_recurrence_bwd(small[0], small[1], b[2], small[3], dlast=small[4])
+    assert all(torch.equal(p, q) for p, q in zip(g, w))
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_refusals(dev):
     x = torch.zeros(4, 2, 6, device=dev)
     h0 = torch.zeros(2, 6, device=dev)

@@ -563,6 +563,27 @@ def test_refusals(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [65, 1500, 9000, 70001])
+def test_far_rows(V):
+    """Rows more than 2^31 elements apart, logits and gradient."""
+    N, far = 3, (1 << 30) + 7
+    buf = torch.empty(2 * far + V, dtype=BF16, device="cuda")
+    z = torch.as_strided(buf, (N, V), (far, 1))
+    z.copy_(rows(N, V, BF16, "cuda"))
+    near = z.contiguous()
+    u = torch.rand(N, device="cuda")
+    for a, b in zip(O.top_logits(z, 5), O.top_logits(near, 5)):
+        assert torch.equal(a, b)
+    values, indices, lse = record(near, 5, 1.0)
+    out = torch.as_strided(torch.empty(2 * far + V, dtype=BF16, device="cuda"), (N, V), (far, 1))
+    a = O.distill_xent(z, values, indices, top_lse=lse, grad=out)
+    b = O.distill_xent(near, values, indices, top_lse=lse)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for kw in (dict(top_k=20), dict(top_p=0.9), dict()):
+        assert torch.equal(O.sample_logits(z, u, **kw), O.sample_logits(near, u, **kw))
+
+
+@pytest.mark.gpu
 def test_refuses_more_rows_than_a_launch_holds():
     z = torch.zeros(1, 3, device="cuda").expand(1 << 22, 3)
     with pytest.raises(RuntimeError):
