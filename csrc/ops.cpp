@@ -2074,17 +2074,28 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linrec_bwd(
   return {dx, df, dh0};
 }
 
+// (no [1, B, H] views of the arguments: two of them cost as much as the launch)
 at::Tensor linrec_step(const at::Tensor& x, const at::Tensor& f, at::Tensor& h,
                        const c10::optional<at::Tensor>& starts) {
-  TORCH_CHECK(x.dim() == 2 && f.dim() == 2, "linrec_step: x and f must be [B, H]");
-  c10::optional<at::Tensor> st;
-  if (has(starts)) {
-    TORCH_CHECK(starts->dim() == 1, "linrec_step: starts must be [B]");
-    st = starts->unsqueeze(0);
-  }
-  dcr::LinrecArgs a = linrec_args(x.unsqueeze(0), f.unsqueeze(0), c10::nullopt, st, "linrec_step");
+  check_f32_or_bf16(x, "x");
+  TORCH_CHECK(x.dim() == 2, "linrec_step: x must be [B, H]");
+  check_on(f, x, x.scalar_type(), "f");
+  TORCH_CHECK(f.sizes() == x.sizes(), "linrec_step: f must be ", x.sizes(), ", got ", f.sizes());
+  TORCH_CHECK(x.size(1) == 1 || (x.stride(1) == 1 && f.stride(1) == 1),
+              "linrec_step: x and f need unit stride along their last dimension");
+  TORCH_CHECK(x.size(0) <= (1 << 28) && x.size(1) <= (1 << 28) &&
+                  x.size(0) * x.size(1) <= (1LL << 28), "linrec_step: at most 2^28 channels");
   check_on(h, x, at::kFloat, "h");
   TORCH_CHECK(h.sizes() == x.sizes() && h.is_contiguous(), "linrec_step: h must be [B, H], contiguous");
+  dcr::LinrecArgs a{};
+  a.T = 1; a.B = (int)x.size(0); a.H = (int)x.size(1);
+  a.x = x.data_ptr(); a.x_b = x.stride(0);
+  a.f = f.data_ptr(); a.f_b = f.stride(0);
+  if (has(starts)) {
+    check_on(*starts, x, at::kBool, "starts");
+    TORCH_CHECK(starts->dim() == 1 && starts->size(0) == a.B, "linrec_step: starts must be [B]");
+    a.starts = ptr<unsigned char>(*starts); a.starts_b = starts->stride(0);
+  }
   OnDevice dev(x);
   at::Tensor y = linrec_out(x);
   if (x.numel() == 0) return y;

@@ -185,9 +185,9 @@ __device__ __forceinline__ unsigned long long wave_scan(unsigned long long x) {
   return x;
 }
 
-// Over a workgroup of NT threads; `red` holds NT / 64 entries.  Every thread gets the result.
-// KEEP: `red` is not used again before another barrier, so none follows.
-template <int NT, bool KEEP = false, typename T, typename F>
+// Over a workgroup of NT threads; `red` holds NT / 64 entries.  Every thread gets the result, and
+// `red` is free again.
+template <int NT, typename T, typename F>
 __device__ __forceinline__ T block_reduce(T x, T* red, F&& op) {
   x = wave_reduce(x, op);
   if constexpr (NT == 64) return x;
@@ -196,7 +196,7 @@ __device__ __forceinline__ T block_reduce(T x, T* red, F&& op) {
   T r = red[0];
 #pragma unroll
   for (int i = 1; i < NT / 64; ++i) r = op(r, red[i]);
-  if (!KEEP) __syncthreads();
+  __syncthreads();
   return uniform(r);
 }
 // Several at once, one barrier: x[i] of K values with the same op; `red` holds K * NT / 64.
