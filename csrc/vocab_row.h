@@ -83,7 +83,8 @@ struct Row {
           if (bits >> j & 1) q[c][j] = (T)-INFINITY;
     }
   }
-  __device__ __forceinline__ int chunks() const { return kChunks; }
+  // the ones that visit() comes to
+  __device__ __forceinline__ int chunks() const { return (V + NT * 4 - 1) / (NT * 4); }
 };
 template <typename T, int NT>
 struct Row<T, NT, 0> {

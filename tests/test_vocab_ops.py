@@ -445,6 +445,22 @@ def test_sample_many_rows(N, V, dtype):
         assert torch.equal(got.cpu(), O.sample_logits(z.cpu(), u, **kw)), kw
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [257, 300, 511, 512, 513, 768, 769])
+def test_sample_rows_that_leave_chunks_empty(V, dtype):
+    """Rows of one wave that do not fill its last chunks: the draw's running weights have no part of
+    them.  Between the draws other rows of the same kernel leave theirs behind in LDS."""
+    N = 4000
+    full = rows(N, 1024, dtype, "cuda", seed=V)
+    u = torch.rand(N, generator=torch.Generator().manual_seed(V))
+    for i, kw in enumerate([dict(), dict(min_p=0.01), dict(top_p=0.9), dict(temperature=30.0)]):
+        z = rows(N, V, dtype, "cuda", seed=i, pad=i % 2)
+        O.sample_logits(full, u.cuda())
+        got = O.sample_logits(z, u.cuda(), **kw)
+        assert torch.equal(got.cpu(), O.sample_logits(z.cpu(), u, **kw)), kw
+
+
 @pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("V", [5, 65, 300, 1500, 5000])
 def test_sample_hard_rows(V, dev):
