@@ -80,6 +80,12 @@ template <bool MARKS>
 __device__ __forceinline__ float step_(float a, float h, float b) {
   return MARKS && a == 0.f ? b : __builtin_fmaf(a, h, b);
 }
+// The factor of two stretches together: a start in either cuts both, whatever the other holds (a NaN
+// gate times zero would be a NaN).
+template <bool MARKS>
+__device__ __forceinline__ float both(float p, float a) {
+  return MARKS && (p == 0.f || a == 0.f) ? 0.f : p * a;
+}
 
 struct Lane {  // one lane's VEC channels
   bool on;
@@ -170,10 +176,12 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
     float A[VEC], B[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) A[j] = 1.f, B[j] = 0.f;
+    bool cut = false;  // a start among the wave's steps
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       const bool live = t0 + i < l.len;
       const bool start = MARKS && st && st[(long)min(t0 + i, p.T - 1) * p.starts_t];
+      cut |= live && start;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float keep, take;
@@ -186,7 +194,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
     }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      sA[buf][w][lane * VEC + j] = A[j];
+      sA[buf][w][lane * VEC + j] = MARKS && cut ? 0.f : A[j];
       sB[buf][w][lane * VEC + j] = B[j];
     }
     __syncthreads();  // (the other buffer's readers passed the previous tile's barrier)
@@ -203,7 +211,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
         if (ww == w) h[j] = carry[j];
         const float aa = sA[buf][ww][lane * VEC + j];
         carry[j] = step_<MARKS>(aa, carry[j], sB[buf][ww][lane * VEC + j]);
-        if (SUMMARY) pa[j] *= aa;
+        if (SUMMARY) pa[j] = both<MARKS>(pa[j], aa);
       }
     if (!SUMMARY) {
 #pragma unroll
@@ -296,7 +304,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
         G[j] = (MARKS && (cut >> i & 1)) ? 0.f : keep[i][j] * (g[i][j] + G[j]);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      sA[buf][w][lane * VEC + j] = A[j];
+      sA[buf][w][lane * VEC + j] = MARKS && cut ? 0.f : A[j];
       sG[buf][w][lane * VEC + j] = G[j];
       if (!SUMMARY) sB[buf][w][lane * VEC + j] = B[j];
     }
@@ -318,7 +326,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
         if (ww == w) ein[j] = e[j];
         const float aa = sA[buf][ww][lane * VEC + j];
         e[j] = step_<MARKS>(aa, e[j], sG[buf][ww][lane * VEC + j]);
-        if (SUMMARY) pa[j] *= aa;
+        if (SUMMARY) pa[j] = both<MARKS>(pa[j], aa);
       }
     if (!SUMMARY) {
       float hp[kC][VEC];  // the state that step i multiplies

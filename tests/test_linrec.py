@@ -200,6 +200,80 @@ def test_padding_and_starts_let_nothing_through(dtype, dev):
     assert torch.equal(g2[0][9:, 0], cg[0][9:, 0]) and torch.equal(g2[1][9:, 0], cg[1][9:, 0])
 
 
+def documents(T, B, dev, every=37):
+    """Starts at places that differ from stream to stream, in neighbouring steps too; the last stream
+    begins in a document that goes on from before.  With the first and the last step of the document
+    that each step belongs to, [T, B]."""
+    starts = torch.zeros(T, B, dtype=torch.bool)
+    for b in range(B):
+        starts[b % 5::every + 4 * b, b] = True
+        starts[min(b % 5 + 1, T - 1), b] = True
+    starts[:every, B - 1] = False
+    starts[T // 2, B - 1] = True
+    first = torch.zeros(T, B, dtype=torch.long)
+    last = torch.zeros(T, B, dtype=torch.long)
+    for t in range(T):
+        first[t] = torch.where(starts[t], t, first[max(t - 1, 0)])
+    for t in reversed(range(T)):
+        last[t] = T - 1 if t == T - 1 else torch.where(starts[t + 1], t, last[t + 1])
+    return starts.to(dev), first, last
+
+
+def check_nan_stays_in_its_document(T, B, H, dtype, dev, level):
+    """One NaN a channel, next to a start and far from one.  What depends on it is NaN -- from there to
+    the document's last step forward, to its first backward -- and all else as without it."""
+    x, f, h0, dh, dlast = inputs(T, B, H, dtype, dev)
+    f = f + level
+    starts, first, last = documents(T, B, dev)
+    clean = R.linear_recurrence_fwd(x, f, h0, starts=starts)
+    cg = R.linear_recurrence_bwd(x, f, clean[2], dh, dlast=dlast, starts=starts)
+    g = torch.Generator().manual_seed(9)
+    at = torch.randint(0, T, (B, H), generator=g)
+    marked = starts.cpu()
+    for b in range(B):  # three channels of four within a step of a start
+        near = marked[:, b].nonzero()[:, 0]
+        pick = near[torch.randint(0, len(near), (H,), generator=g)] + torch.arange(H) % 4 - 1
+        at[b] = torch.where(torch.arange(H) % 4 < 3, pick.clamp(0, T - 1), at[b])
+    steps = torch.arange(T)[:, None, None]
+    s = first.gather(0, at.t().reshape(-1, B).contiguous()).t()  # [B, H]: of the NaN's document
+    e = last.gather(0, at.t().reshape(-1, B).contiguous()).t()
+    after, until = (steps >= at) & (steps <= e), (steps >= s) & (steps <= at)
+    inside, none = (steps >= s) & (steps <= e), torch.zeros(T, B, H, dtype=torch.bool)
+    open_ = (s == 0) & ~marked[0][:, None]  # the document goes on from h0
+    want = dict(x=(after, none, after), f=(after, until, inside), dh=(none, until, until))
+    for what, (h_nan, dx_nan, df_nan) in want.items():
+        v = dict(x=x, f=f, dh=dh)
+        v[what] = v[what].clone()
+        v[what].scatter_(0, at[None].to(dev), float("nan"))
+        h, end, carry = R.linear_recurrence_fwd(v["x"], v["f"], h0, starts=starts)
+        dx, df, dh0 = R.linear_recurrence_bwd(v["x"], v["f"], carry, v["dh"], dlast=dlast,
+                                              starts=starts)
+        for name, got, ref, nan in (("h", h, clean[0], h_nan), ("final", end, clean[1], h_nan[-1]),
+                                    ("dx", dx, cg[0], dx_nan), ("df", df, cg[1], df_nan),
+                                    ("dh0", dh0, cg[2], dx_nan[0] & open_)):
+            nan = nan.to(dev)
+            assert torch.equal(got.isnan(), nan), (what, name)
+            assert torch.equal(got[~nan], ref[~nan]), (what, name)
+
+
+NAN_SHAPES = [(9, 2, 16), (41, 4, 20), (200, 2, 33)]
+# these are cut into segments, of one, two and four channels a lane
+NAN_SHAPES_LONG = [(1100, 2, 24), (2100, 3, 1000), (4400, 3, 1000)]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("T,B,H", NAN_SHAPES)
+def test_nan_gates_stay_in_their_document(T, B, H, dev):
+    check_nan_stays_in_its_document(T, B, H, F32, dev, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,B,H", NAN_SHAPES_LONG)
+def test_nan_gates_stay_in_their_document_long(T, B, H, dtype):
+    check_nan_stays_in_its_document(T, B, H, dtype, "cuda", 0.0)
+
+
 @pytest.mark.parametrize("dev", DEVS)
 def test_saturated_gates(dev):
     """Gates at the ends of the range: the state is kept or replaced to the last digit."""
