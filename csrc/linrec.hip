@@ -75,16 +75,20 @@ __device__ __forceinline__ void gates(float f, float& keep, float& take) {
   keep = f >= 0.f ? r : t * r;
   take = f >= 0.f ? t * r : r;
 }
-// a h + b; with MARKS a factor of zero (a start) lets nothing of h through, not even a NaN
+// The factor of a start, and of every stretch with one: it lets nothing through, not even a NaN.  No
+// product of gates is -0, so a gate or a product that is too small for a number stays apart from it,
+// and a NaN state goes through that.
+constexpr float kCut = -0.0f;
+__device__ __forceinline__ bool is_cut(float a) { return __float_as_uint(a) == 0x80000000u; }
+// a h + b
 template <bool MARKS>
 __device__ __forceinline__ float step_(float a, float h, float b) {
-  return MARKS && a == 0.f ? b : __builtin_fmaf(a, h, b);
+  return MARKS && is_cut(a) ? b : __builtin_fmaf(a, h, b);
 }
-// The factor of two stretches together: a start in either cuts both, whatever the other holds (a NaN
-// gate times zero would be a NaN).
+// The factor of two stretches together.
 template <bool MARKS>
 __device__ __forceinline__ float both(float p, float a) {
-  return MARKS && (p == 0.f || a == 0.f) ? 0.f : p * a;
+  return MARKS && (is_cut(p) || is_cut(a)) ? kCut : p * a;
 }
 
 struct Lane {  // one lane's VEC channels
@@ -186,7 +190,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
       for (int j = 0; j < VEC; ++j) {
         float keep, take;
         gates(a[i][j], keep, take);
-        a[i][j] = !live ? 1.f : start ? 0.f : keep;
+        a[i][j] = !live ? 1.f : start ? kCut : keep;
         b[i][j] = live ? take * b[i][j] : 0.f;
         B[j] = step_<MARKS>(a[i][j], B[j], b[i][j]);
         A[j] *= a[i][j];
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
     }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      sA[buf][w][lane * VEC + j] = MARKS && cut ? 0.f : A[j];
+      sA[buf][w][lane * VEC + j] = MARKS && cut ? kCut : A[j];
       sB[buf][w][lane * VEC + j] = B[j];
     }
     __syncthreads();  // (the other buffer's readers passed the previous tile's barrier)
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
         gates(keep[i][j], keep[i][j], take[i][j]);
         if (!live) keep[i][j] = 1.f, take[i][j] = 0.f, g[i][j] = 0.f;
         if (!live && !SUMMARY) xv[i][j] = 0.f;
-        const float a = (MARKS && (cut >> i & 1)) ? 0.f : keep[i][j];
+        const float a = (MARKS && (cut >> i & 1)) ? kCut : keep[i][j];
         if (!SUMMARY) B[j] = step_<MARKS>(a, B[j], take[i][j] * xv[i][j]);
         A[j] *= a;
       }
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
         G[j] = (MARKS && (cut >> i & 1)) ? 0.f : keep[i][j] * (g[i][j] + G[j]);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      sA[buf][w][lane * VEC + j] = MARKS && cut ? 0.f : A[j];
+      sA[buf][w][lane * VEC + j] = MARKS && cut ? kCut : A[j];
       sG[buf][w][lane * VEC + j] = G[j];
       if (!SUMMARY) sB[buf][w][lane * VEC + j] = B[j];
     }

@@ -219,12 +219,12 @@ def documents(T, B, dev, every=37):
     return starts.to(dev), first, last
 
 
-def check_nan_stays_in_its_document(T, B, H, dtype, dev, level):
+def check_nan_stays_in_its_document(T, B, H, dtype, dev, level, every=37):
     """One NaN a channel, next to a start and far from one.  What depends on it is NaN -- from there to
     the document's last step forward, to its first backward -- and all else as without it."""
     x, f, h0, dh, dlast = inputs(T, B, H, dtype, dev)
     f = f + level
-    starts, first, last = documents(T, B, dev)
+    starts, first, last = documents(T, B, dev, every)
     clean = R.linear_recurrence_fwd(x, f, h0, starts=starts)
     cg = R.linear_recurrence_bwd(x, f, clean[2], dh, dlast=dlast, starts=starts)
     g = torch.Generator().manual_seed(9)
@@ -272,6 +272,41 @@ def test_nan_gates_stay_in_their_document(T, B, H, dev):
 @pytest.mark.parametrize("T,B,H", NAN_SHAPES_LONG)
 def test_nan_gates_stay_in_their_document_long(T, B, H, dtype):
     check_nan_stays_in_its_document(T, B, H, dtype, "cuda", 0.0)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("T,B,H", NAN_SHAPES)
+def test_nan_outlives_small_products(T, B, H, dev):
+    """Gates whose product over eight steps is too small for fp32 (exp(-112)) are no starts."""
+    check_nan_stays_in_its_document(T, B, H, F32, dev, -15.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,B,H,level", [s + (-15.0,) for s in NAN_SHAPES_LONG]
+                         + [(40000, 1, 64, -1.0), (12000, 4, 360, -1.0)])
+def test_nan_outlives_small_products_long(T, B, H, level):
+    """Level -1: gates around a half, whose product over a segment's 200 steps or more is too small;
+    documents of many segments."""
+    check_nan_stays_in_its_document(T, B, H, F32, "cuda", level, every=max(37, T // 7))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("T,level", [(50, -14.0), (1300, -4.0)])
+def test_marks_lose_no_bad_state(T, level, bad, dev):
+    """A state or a gradient that is not finite stays so with lengths given, as it does without."""
+    B, H = 2, 12
+    x, f, h0, dh, dlast = inputs(T, B, H, F32, dev)
+    f = torch.full_like(f, level)
+    h0[0, 3], dlast[1, 5] = bad, bad
+    lengths = torch.full((B,), T, dtype=torch.int32, device=dev)
+    for n in (None, lengths):
+        h, last, carry = R.linear_recurrence_fwd(x, f, h0, lengths=n)
+        dx, df, dh0 = R.linear_recurrence_bwd(x, f, carry, dh, dlast=dlast, lengths=n)
+        for got, at in ((h[:, 0, 3], True), (last[0, 3], True), (dx[:, 1, 5], True),
+                        (df[:, 1, 5], True), (dh0[1, 5], True), (h[:, 1], False),
+                        (last[1], False), (dx[:, 0], False), (dh0[0], False)):
+            assert (got.isfinite() != at).all()
 
 
 @pytest.mark.parametrize("dev", DEVS)
