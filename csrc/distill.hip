@@ -4,6 +4,7 @@
 // With the student's p = softmax(z / T) and the teacher's recorded entries (i_j, t_j):
 //   q_j = exp(t_j / T - lse), r = max(0, 1 - sum q_j)   with the teacher's log-sum-exp at T, or
 //   q   = softmax_j(t_j / T), r = 0                     without it
+//   no divergence, where all t_j are -inf and the log-sum-exp is, or is not given
 //   loss = alpha T^2 [sum_j q_j (log q_j - log p_{i_j}) + r (log r - log s)]
 //        + (1 - alpha) (lse(z) - z_y),                  s = the student's mass off the entries
 //   d/dz_v = alpha T (p_v - q_v)            at the entries
@@ -179,10 +180,11 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   const float lse = logf(all), inv_all = 1.0f / all, off = sr * wr * inv_all;  // off: s
   const float wr1 = two ? expf(dr) : wr, all1 = two ? sr1 * wr1 + sk1 * expf(dk) : all;
   const bool told = a.lse != nullptr;
-  // entries that hold nothing say nothing
-  const bool mute = !told && mt == -INFINITY;
+  const float tl = told ? a.lse[n] : 0.f;
+  // entries that hold nothing say nothing, unless the teacher's mass lies elsewhere
+  const bool mute = mt == -INFINITY && (!told || tl == -INFINITY);
   // log q = t / T - lt - log st, where without the teacher's log-sum-exp t counts from its maximum
-  const float lt = told ? a.lse[n] : logf(sum[4]), t0 = told ? 0.f : mt;
+  const float lt = told ? tl : logf(sum[4]), t0 = told ? 0.f : mt;
   float q_e[kE], p_e[kE], say[3] = {0.f, 0.f, 0.f};  // sums of q, of the terms, of q - p
 #pragma unroll
   DCR_ENTRIES(e) {

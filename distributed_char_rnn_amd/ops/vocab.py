@@ -75,6 +75,8 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
     An entry whose index is not in ``[0, V)`` is none (rows with fewer than k entries are padded
     with -1); a token recorded twice counts with both values.  A row whose target is not in
     ``[0, V)`` is padding, as is one whose logits are all -inf: loss and gradient are zero there.
+    A record that holds nothing -- all values -inf, and ``top_lse`` too where it is given, as
+    :func:`top_logits` answers to a row of nothing but -inf -- has no divergence.
 
     The gradient is written in ``grad_dtype`` (the logits' by default) or into ``grad``."""
     if scale is None:
@@ -224,11 +226,13 @@ def _cpu_distill_xent(logits, values, indices, lse, targets, alpha, tau, scale, 
     logp = torch.log_softmax(z / tau, 1)
     t = torch.where(here, values / tau, -math.inf)
     some = ~torch.isneginf(t).all(1)
-    logq = t - (lse if lse is not None else torch.where(some, torch.logsumexp(t, 1), 0.0))[:, None]
+    if lse is not None:
+        some = some | ~torch.isneginf(lse)
+    base = torch.logsumexp(t, 1) if lse is None else lse
+    logq = t - torch.where(some, base, 0.0)[:, None]
     q = logq.exp()
     kl = torch.where(q > 0, q * (logq - logp.gather(1, idx)), 0.0).sum(1)
     g = logp.exp()
-    on = torch.ones(n, 1)
     if lse is not None:
         entry = torch.zeros(n, v + 1).scatter_(
             1, torch.where(here, idx, v), 1.0)[:, :v].bool()
@@ -238,10 +242,8 @@ def _cpu_distill_xent(logits, values, indices, lse, targets, alpha, tau, scale, 
         kl = kl + torch.where(left, rest * (rest.log() - out), 0.0)
         gone = torch.where(left, rest.log() - out, -math.inf)[:, None]
         g = torch.where(entry, g, g - torch.where(left[:, None], (logp + gone).exp(), 0.0))
-    else:
-        on = some.float()[:, None]
-        kl = torch.where(some, kl, 0.0)
-    g = (g.scatter_add(1, idx, -torch.where(here, q, 0.0))) * (alpha * tau) * on
+    kl = torch.where(some, kl, 0.0)
+    g = (g.scatter_add(1, idx, -torch.where(here, q, 0.0))) * (alpha * tau) * some.float()[:, None]
     row = alpha * tau * tau * kl
     if targets is not None and alpha < 1:
         y = targets.long().clamp(0, v - 1)[:, None]

@@ -239,6 +239,42 @@ def test_distill_odd_records(V, dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("V", [65, 1500, 40001])
+@pytest.mark.parametrize("alpha", [0.4, 1.0])
+def test_distill_teacher_row_without_tokens(V, alpha, dev):
+    """A teacher's row that its mask leaves empty records -inf throughout: it says nothing, and the
+    target's part of the loss stays."""
+    N, k, tau = 4, 7, 2.0
+    t, z = rows(N, V, F32, dev, seed=1), rows(N, V, F32, dev, seed=2)
+    t[1] = -INF
+    y = torch.randint(0, V, (N,), generator=torch.Generator().manual_seed(1)).int().to(dev)
+    y[3] = -1
+    values, indices, lse = O.top_logits(t, k, tau)
+    assert lse[1] == -INF and (values[1] == -INF).all()
+    for record_of in ((values, indices), (values, torch.where(values > -INF, indices, -1))):
+        _, row, grad = O.distill_xent(z, *record_of, top_lse=lse, targets=y, alpha=alpha,
+                                      temperature=tau)
+        # a finite log-sum-exp and the other rows: as they were
+        want, gwant = reference_distill(z, values, indices, torch.where(lse > -INF, lse, 0.0), y,
+                                        alpha, tau, 1.0 / N)
+        lp = torch.log_softmax(z[1].double().cpu(), 0)
+        want[1] = -(1 - alpha) * lp[int(y[1])]
+        gwant[1] = (1 - alpha) / N * lp.exp()
+        gwant[1, int(y[1])] -= (1 - alpha) / N
+        # as check_distill's bound, with logits and log-probabilities up to 40
+        bound = (2 * 20 + 64 + 2 * k) * U
+        assert ((row.double().cpu() - want).abs() <= bound * (alpha * tau * tau + 1) * 40).all()
+        assert ((grad.double().cpu() - gwant).abs() <= bound * (alpha * tau + 1) / N).all()
+        assert row[3] == 0 and (grad[3] == 0).all()
+        if alpha == 1.0:
+            assert row[1] == 0 and (grad[1] == 0).all()
+    leaf = z.clone().requires_grad_(True)
+    O.distill_loss(leaf, values, indices, top_lse=lse, targets=y, alpha=alpha,
+                   temperature=tau).backward()
+    assert torch.allclose(leaf.grad, grad, atol=1e-9, rtol=1e-6)
+
+
+@pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("tau", [0.5, 2.0])
 def test_distill_lowest_values(tau, dtype, dev):
