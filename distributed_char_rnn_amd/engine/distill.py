@@ -29,9 +29,11 @@ class Teacher:
         self.state = None
 
     @classmethod
-    def load(cls, save_dir: str, chars: Sequence[str], device, **kw) -> "Teacher":
-        """The latest checkpoint of ``save_dir``, whose vocabulary must be the student's."""
-        model, saved, _, _ = load_for_inference(save_dir, device)
+    def load(cls, save_dir: str, chars: Sequence[str], device, dtype: str = "auto",
+             **kw) -> "Teacher":
+        """The latest checkpoint of ``save_dir``, whose vocabulary must be the student's; it computes
+        in ``dtype``, the student's."""
+        model, saved, _, _ = load_for_inference(save_dir, device, dtype)
         if tuple(saved) != tuple(chars):
             raise ValueError(f"the teacher in {save_dir} was trained on another character set")
         return cls(model, **kw)

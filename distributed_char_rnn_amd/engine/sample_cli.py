@@ -21,14 +21,14 @@ from ..utils.config import sample_parser
 from .sampler import sample
 
 
-def load_for_inference(save_dir: str, device="auto"):
+def load_for_inference(save_dir: str, device="auto", dtype: str = "auto"):
     saved = safe_pickle.load(os.path.join(save_dir, "config.pkl"))
     chars, vocab = safe_pickle.load(os.path.join(save_dir, "chars_vocab.pkl"))
     if device == "auto":
         device = "cuda" if torch.cuda.is_available() else "cpu"
     cfg = ModelConfig(model=saved.model, vocab_size=saved.vocab_size, rnn_size=saved.rnn_size,
                       num_layers=saved.num_layers)
-    model = CharRNN(cfg, device=device, seed=0)
+    model = CharRNN(cfg, device=device, seed=0, dtype=dtype)
     prefix = ckpt.latest_checkpoint(save_dir)
     if prefix is None:
         raise FileNotFoundError(f"no checkpoint found in {save_dir}")

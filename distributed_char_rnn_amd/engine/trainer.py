@@ -252,7 +252,8 @@ def _train(args, ctx, device, rank: int, chief: bool) -> int:
              "--save_state): the resumed epoch continues from a zero state", rank)
     teacher = None
     if getattr(args, "teacher", None):
-        teacher = Teacher.load(args.teacher, loader.chars, device, top_k=args.teacher_top_k,
+        teacher = Teacher.load(args.teacher, loader.chars, device,
+                               dtype=getattr(args, "dtype", "auto"), top_k=args.teacher_top_k,
                                alpha=args.distill_alpha, temperature=args.distill_temperature)
         _log(f"distilling from {args.teacher}: top {teacher.k} logits at temperature "
              f"{teacher.temperature:g}, weight {teacher.alpha:g}", rank)

@@ -180,6 +180,42 @@ def test_resume_gives_the_teacher_its_state_back(tmp_path, dev, monkeypatch):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", ["auto", "fp32"])
+def test_teacher_computes_in_the_students_type(tmp_path, dev, dtype, monkeypatch):
+    """``--dtype`` holds for the teacher, too; in fp32 on a GPU its record is the oracle's."""
+    from distributed_char_rnn_amd.engine import trainer
+    from distributed_char_rnn_amd.utils.config import train_parser
+
+    monkeypatch.chdir(tmp_path)
+    common = ["--synthetic_text", "2000", "--batch_size", "4", "--seq_length", "20", "--num_epochs",
+              "1", "--log_dir", "logs", "--summary_every", "0", "--device", dev, "--rnn_size", "64",
+              "--max_steps", "3"]
+    teachers, load = [], Teacher.load.__func__
+    asked = []
+
+    def spy(cls, save_dir, chars, device, dtype="auto", **kw):
+        t = load(cls, save_dir, chars, device, dtype, **kw)
+        asked.append(dtype)
+        teachers.append(t)
+        return t
+
+    monkeypatch.setattr(Teacher, "load", classmethod(spy))
+    assert trainer.train(train_parser().parse_args(common + ["--save_dir", "t"])) == 0
+    assert trainer.train(train_parser().parse_args(
+        common + ["--save_dir", "s", "--teacher", "t", "--dtype", dtype])) == 0
+    (t,) = teachers
+    assert asked == [dtype]
+    want = {"cpu": {"auto": "reference", "fp32": "reference"},
+            "cuda": {"auto": "native", "fp32": "native32"}}[dev][dtype]
+    assert t.model.backend_name == want
+    if dtype == "fp32":
+        x, _ = batch(4, 20, t.model.cfg.vocab_size, dev)
+        logits, _ = t.model.backend.sequence_logits(x, t.model.zero_state(4))
+        oracle, _ = ReferenceBackend(t.model.store).sequence_logits(x, t.model.zero_state(4))
+        assert torch.allclose(logits, oracle, rtol=1e-4, atol=1e-5)
+
+
 # ---- sampling ---------------------------------------------------------------------------------
 CHARS = [" "] + [chr(97 + i) for i in range(25)]
 
