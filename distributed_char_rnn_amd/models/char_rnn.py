@@ -96,7 +96,10 @@ class CharRNN:
         # sums to one launch at the end of the step instead of flushing per bucket
         cb = (grad_sync.ready if grad_sync is not None and getattr(grad_sync, "enabled", True)
               else None)
-        kw = {} if distill is None else {"distill": distill}
+        kw = {}
+        if distill is not None:
+            distill.check(xi.shape[1], xi.shape[0])
+            kw["distill"] = distill
         return self.backend.train_step(xi, yi, state, cb, want_extras=want_extras, **kw)
 
     def step_logits(self, x_t, state: State):

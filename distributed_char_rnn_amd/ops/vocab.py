@@ -38,6 +38,20 @@ class Distill(NamedTuple):
     alpha: float
     temperature: float
 
+    def check(self, T: int, B: int) -> None:
+        """Raises unless the record is one of a batch of ``B`` sequences of ``T``: a batch-major one
+        has as many rows, in another order."""
+        v, want = self.values, (T, B)
+        if v.dim() != 3 or tuple(v.shape[:2]) != want:
+            raise ValueError(f"a record's values must be [T, B, k] = [{T}, {B}, k], "
+                             f"got {list(v.shape)}")
+        if self.indices.shape != v.shape:
+            raise ValueError(f"a record's indices must be {list(v.shape)} as its values, "
+                             f"got {list(self.indices.shape)}")
+        if self.lse is not None and tuple(self.lse.shape) != want:
+            raise ValueError(f"a record's lse must be [T, B] = [{T}, {B}], "
+                             f"got {list(self.lse.shape)}")
+
 
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0
                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

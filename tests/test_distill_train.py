@@ -148,6 +148,25 @@ def test_teacher_refuses():
 
 
 @pytest.mark.parametrize("dev", DEVS)
+def test_train_step_refuses_records_of_another_shape(dev):
+    """Batch-major records, of another batch, or with parts of another: as many rows or not."""
+    t, s = models("lstm", 32, 29, dev)
+    x, y = batch(4, 6, 29, dev)
+    d = Teacher(t, top_k=5).record(x)
+    assert d.values.shape == (6, 4, 5)
+    swap = {n: getattr(d, n).transpose(0, 1).contiguous() for n in ("values", "indices", "lse")}
+    for bad in (d._replace(**swap), d._replace(values=swap["values"]),
+                d._replace(indices=swap["indices"]), d._replace(lse=swap["lse"]),
+                d._replace(values=d.values.view(24, 5), indices=d.indices.view(24, 5)),
+                d._replace(indices=d.indices[..., :3]), d._replace(lse=d.lse.view(-1)),
+                Teacher(t, top_k=5).record(x[:2])):
+        with pytest.raises(ValueError, match="record"):
+            s.train_step(x, y, s.zero_state(4), distill=bad)
+    s.train_step(x, y, s.zero_state(4), distill=d._replace(lse=None))
+    s.check_errors()
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_resume_gives_the_teacher_its_state_back(tmp_path, dev, monkeypatch):
     """A run resumed in the middle of an epoch sees the records of the uninterrupted run."""
     from distributed_char_rnn_amd.engine import trainer
