@@ -174,8 +174,8 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     Every setting is a number, or a tensor with one per row (fp32; ``top_k`` int32), where
     ``top_k`` below 1 and NaN mean no filter, ``top_p`` below 0 counts as 0, ``min_p`` above 1 as
     1, and a temperature below 0 or NaN as 0.  NaN logits count as -inf; a row of nothing else
-    gives 0.  Weights are 64-bit, so the answer does not depend on the order of
-    any sum."""
+    gives 0.  Weights are added as whole numbers of 2^-44 of the first's, so the answer does not
+    depend on the order of any sum; a token that weighs less than half of that is never drawn."""
     if not logits.is_cuda:
         return _cpu_sample(logits, u, temperature, top_k, top_p, min_p)
     t, ts = _setting(temperature, 1.0)
@@ -299,14 +299,16 @@ def _cpu_sample(logits, u, temperature, top_k, top_p, min_p):
     w = torch.exp((zs - top) / torch.where(temp > 0, temp, 1.0))
     w = torch.where(zs == top, 1.0, torch.where(torch.isneginf(zs) | torch.isposinf(top), 0.0, w))
     rank = torch.arange(v)[None]
-    w = torch.where((k <= 0) | (rank < k), w, 0.0)
-    before = torch.cumsum(w, 1) - w
-    keep = ~(p < 1) | (rank == 0) | (before < p * w.sum(1, keepdim=True))
+    units = torch.round(w * 2.0 ** 44).long()
+    units = torch.where((k <= 0) | (rank < k), units, 0)
+    before = torch.cumsum(units, 1) - units
+    share = torch.ceil(torch.where(p < 1, p, 1.0).clamp_min(0.0) * units.sum(1, keepdim=True).double())
+    keep = ~(p < 1) | (rank == 0) | (before < share.long())
     keep &= ~(w < q) | (rank == 0)
-    w = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0.0))
-    cdf = torch.cumsum(w, 1)
+    units = torch.zeros_like(units).scatter_(1, order, torch.where(keep, units, 0))
+    cdf = torch.cumsum(units, 1)
+    total = cdf[:, -1:].contiguous()
     r = u.double()[:, None]
-    r = torch.where(r > 0, r, 0.0) * cdf[:, -1:]
-    last = torch.where(w > 0, rank, 0).max(1, keepdim=True).values
-    pick = torch.minimum(torch.searchsorted(cdf, r, right=True), last)
+    r = torch.minimum((torch.where(r > 0, r, 0.0).clamp_max(1.0) * total.double()).long(), total - 1)
+    pick = torch.searchsorted(cdf, r, right=True)
     return torch.where(first, order[:, :1], pick)[:, 0].to(torch.int32)

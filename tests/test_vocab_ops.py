@@ -481,6 +481,27 @@ def test_sample_many_rows(N, V, dtype):
         assert torch.equal(got.cpu(), O.sample_logits(z.cpu(), u, **kw)), kw
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("V", [3, 65, 700, 1500, 20000])
+def test_sample_weights_that_round_to_nothing(V, dev):
+    """The smallest u takes the first token that weighs anything: less than 2^-45 of the largest is
+    nothing (exp(-40) = 2^-57.7), more is something (exp(-30) = 2^-43.3)."""
+    z = torch.full((4, V), -40.0, device=dev)
+    z[:, 2] = 0.0
+    z[1, 1] = -30.0
+    z[2, 0] = -30.0
+    z[3, :2] = torch.tensor([-INF, -80.0])
+    for kw in (dict(), dict(top_k=3), dict(top_k=V), dict(top_p=1 - 2.0 ** -24), dict(min_p=1e-20),
+               dict(temperature=0.5)):
+        got = O.sample_logits(z, torch.zeros(4, device=dev), **kw)
+        if kw in (dict(temperature=0.5), dict(top_p=1 - 2.0 ** -24)):
+            # exp(-60) is nothing; a share of 1 - 2^-24 leaves out what lies behind the first
+            want = [2, 2, 2, 2]
+        else:
+            want = [2, 1, 0, 2]
+        assert got.tolist() == want, kw
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [257, 300, 511, 512, 513, 768, 769])
