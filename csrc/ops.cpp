@@ -2151,6 +2151,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logi
   return {values, indices, lse};
 }
 
+// Rows [N, V] of `b` that may be written while those of `a` are read: the very same memory (a thread
+// writes the columns that it has read), or none of it.  Rows of two views of one buffer can lie side
+// by side: with the same row stride, they are apart by the remainder of their distance.
+bool rows_apart_or_same(const at::Tensor& a, const at::Tensor& b) {
+  const int64_t N = a.size(0), V = a.size(1), ea = a.element_size(), eb = b.element_size();
+  if (!a.is_alias_of(b) || a.numel() == 0) return true;
+  const int64_t la = (N > 1 ? a.stride(0) : 0) * ea, lb = (N > 1 ? b.stride(0) : 0) * eb;
+  const int64_t d = (int64_t)((const char*)b.data_ptr() - (const char*)a.data_ptr());
+  if (d >= (N - 1) * la + V * ea || -d >= (N - 1) * lb + V * eb) return true;
+  if (la != lb || ea != eb) return false;
+  if (d == 0) return true;
+  if (la == 0) return false;  // (one row, or one that is read for all)
+  const int64_t r = (d % la + la) % la;
+  return r >= V * ea && la - r >= V * ea;
+}
+
 void distill(const at::Tensor& logits, const at::Tensor& values, const at::Tensor& indices,
              const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& targets,
              double alpha, double temperature, double scale,
@@ -2188,6 +2204,8 @@ void distill(const at::Tensor& logits, const at::Tensor& values, const at::Tenso
                     (a.r.V == 1 || grad->stride(1) == 1) && (a.r.N <= 1 || grad->stride(0) >= a.r.V),
                 "distill: grad must be [N, V] on the logits' device, unit stride along the "
                 "vocabulary, rows apart");
+    TORCH_CHECK(rows_apart_or_same(logits, *grad),
+                "distill: grad must be the logits' own memory, in their type, or share none of it");
     a.grad = grad->data_ptr(); a.grad_ld = grad->stride(0);
     a.grad_bf16 = grad->scalar_type() == at::kBFloat16;
   }

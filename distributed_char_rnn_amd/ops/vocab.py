@@ -92,7 +92,8 @@ def distill_xent(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tens
     A record that holds nothing -- all values -inf, and ``top_lse`` too where it is given, as
     :func:`top_logits` answers to a row of nothing but -inf -- has no divergence.
 
-    The gradient is written in ``grad_dtype`` (the logits' by default) or into ``grad``."""
+    The gradient is written in ``grad_dtype`` (the logits' by default) or into ``grad``, which may
+    be the logits themselves, but else shares no memory with them."""
     if scale is None:
         scale = 1.0 / max(1, logits.shape[0])
     if not logits.is_cuda:

@@ -382,6 +382,54 @@ def test_distill_autograd_and_differences(dtype, dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,V", [(5, 65), (4, 1500), (1100, 1500), (3, 9000), (1100, 9000), (3, 40001)])
+def test_distill_gradient_over_the_logits(N, V, dtype, dev):
+    """The gradient written over the logits, with entries and targets everywhere in the row, and beside
+    them in the rows of one buffer."""
+    k = 9
+    buf = rows(N, 2 * V + 3, dtype, dev)
+    z = buf[:, 1:V + 1]
+    g = torch.Generator().manual_seed(6)
+    y = torch.randint(0, V, (N,), generator=g).int().to(dev)
+    indices = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(N)]).int().to(dev)
+    values = torch.randn(N, k, generator=g).to(dev)
+    kw = dict(targets=y, alpha=0.6, temperature=2.0)
+    want = O.distill_xent(z, values, indices, **kw)
+    beside = O.distill_xent(z, values, indices, grad=buf[:, V + 1:2 * V + 1], **kw)
+    over = O.distill_xent(z, values, indices, grad=z, **kw)
+    for got in (beside, over):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert over[2].data_ptr() == z.data_ptr()
+
+
+@pytest.mark.gpu
+def test_distill_refuses_a_gradient_across_the_logits():
+    N, V, k = 4, 65, 3
+    buf = rows(N, 3 * V, F32, "cuda")
+    flat = torch.zeros(4 * N * V, device="cuda")
+    z = buf[:, V:2 * V]
+    values, indices, _ = O.top_logits(z.contiguous(), k)
+    for grad in (buf[:, V + 1:2 * V + 1], buf[:, 1:V + 1], buf[:, V - 3:2 * V - 3]):
+        with pytest.raises(RuntimeError, match="memory"):
+            O.distill_xent(z, values, indices, grad=grad)
+    a = flat[:N * V].view(N, V)
+    for off, ok in ((0, True), (1, False), (N * V - 1, False), (N * V, True), (V, False)):
+        b = flat[off:off + N * V].view(N, V)
+        for p, q in ((a, b), (b, a)):
+            if ok:
+                O.distill_xent(p, values, indices, grad=q)
+            else:
+                with pytest.raises(RuntimeError, match="memory"):
+                    O.distill_xent(p, values, indices, grad=q)
+    half = flat.view(BF16)[:N * V].view(N, V)  # the same place in another type
+    with pytest.raises(RuntimeError, match="memory"):
+        O.distill_xent(a, values, indices, grad=half)
+    with pytest.raises(RuntimeError, match="memory"):
+        O.distill_xent(a[:1].expand(N, V), values, indices, grad=a)
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_distill_agrees_with_cross_entropy(dev):
     """A record of one sure entry is a target: the loss is the plain cross-entropy."""
     N, V = 8, 65
