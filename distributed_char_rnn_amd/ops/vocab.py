@@ -206,7 +206,9 @@ def _check_logits(logits):
 
 
 def _check_temperature(t):
-    torch._check(t > 0 and math.isfinite(t), lambda: "the temperature must be positive and finite")
+    both = torch.tensor([t, 1.0 / t if t > 0 else 0.0], dtype=torch.float64).float()  # as used
+    torch._check(bool((both > 0).all() and both.isfinite().all()),
+                 lambda: f"the temperature must be positive and finite, got {t}")
 
 
 def _check_rows(t, logits, dtype, shape, name):
@@ -226,6 +228,13 @@ def _cpu_distill_xent(logits, values, indices, lse, targets, alpha, tau, scale, 
     ok(0 <= alpha <= 1, lambda: "alpha must be in [0, 1]")
     ok(alpha == 1 or targets is not None, lambda: "alpha < 1 needs targets")
     ok(math.isfinite(scale), lambda: "scale must be finite")
+    kind = (grad_dtype or logits.dtype) if grad is None else grad.dtype
+    ok(kind in (torch.float32, torch.bfloat16), lambda: "grad must be float32 or bfloat16")
+    if grad is not None:
+        ok(grad.device == logits.device and grad.shape == logits.shape
+           and (v == 1 or grad.stride(1) == 1) and (n <= 1 or grad.stride(0) >= v),
+           lambda: "grad must be [N, V] on the logits' device, unit stride along the vocabulary, "
+                   "rows apart")
     z = logits.float()
     idx = indices.long()
     here = (idx >= 0) & (idx < v)

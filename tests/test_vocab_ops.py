@@ -683,6 +683,23 @@ def test_refusals(dev):
             pytest.fail(f"call {n} was not refused")
 
 
+@pytest.mark.parametrize("dev", DEVS)
+def test_refusals_are_the_same_on_both_devices(dev):
+    z = rows(4, 65, F32, dev)
+    v, i, lse = O.top_logits(z, 4)
+    wide = torch.zeros(4, 65, device=dev)
+    for t in (1e-46, 1e-40, 1e39, 1e300, NAN):  # no number, or no reciprocal, in fp32
+        for call in (lambda: O.top_logits(z, 4, t), lambda: O.distill_xent(z, v, i, temperature=t)):
+            with pytest.raises(RuntimeError):
+                call()
+    for kw in (dict(grad_dtype=torch.float16), dict(grad_dtype=torch.float64),
+               dict(grad=wide.half()), dict(grad=wide.double()), dict(grad=wide[:2]),
+               dict(grad=wide[None]), dict(grad=wide[:, :64]), dict(grad=wide[:1].expand(4, 65)),
+               dict(grad=torch.zeros(65, 4, device=dev).t())):
+        with pytest.raises(RuntimeError):
+            O.distill_xent(z, v, i, top_lse=lse, **kw)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("V", [65, 1500, 9000, 70001])
 def test_far_rows(V):
