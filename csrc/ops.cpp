@@ -2500,6 +2500,11 @@ TORCH_LIBRARY(dcr, m) {
         "bool want_carry) -> (Tensor, Tensor, Tensor)");
   m.def("linrec_bwd(Tensor x, Tensor f, Tensor carry, Tensor dh, Tensor? dlast, Tensor? lengths, "
         "Tensor? starts) -> (Tensor, Tensor, Tensor)");
+  m.def("linrec_plan(int T, int B, int H) -> int[]",
+        [](int64_t T, int64_t B, int64_t H) -> std::vector<int64_t> {
+          const dcr::LinrecPlan q = dcr::linrec_plan((int)T, (int)B, (int)H);
+          return {q.vec, q.waves, q.tiles, q.segs, q.tiles_per_seg};
+        });
   m.def("linrec_step(Tensor x, Tensor f, Tensor(a!) h, Tensor? starts) -> Tensor");
   m.def("top_logits(Tensor logits, int k, float temperature) -> (Tensor, Tensor, Tensor)");
   m.def("distill(Tensor logits, Tensor values, Tensor indices, Tensor? lse, Tensor? targets, "
