@@ -388,3 +388,124 @@ def test_linear_student(dtype, dev):
             assert torch.allclose(o.float(), full.view(T, B, V)[t].float(), atol=tol, rtol=tol)
             pick = O.sample_logits(o.float(), u[t], 0.8, 10, 0.9)
             assert ((pick >= 0) & (pick < V)).all()
+
+
+# ---- modes of training with a teacher ---------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("model,H", [("lstm", 64), ("gru", 48), ("rnn", 32)])
+def test_fp32_step_matches_oracle(model, H):
+    """``--dtype fp32``: teacher and student on the fp32 kernels, loss and gradients at fp32 accuracy
+    (as the cross-entropy step's, tests/test_fp32.py)."""
+    V, B, T = 65, 6, 11
+    t = CharRNN(ModelConfig(model="lstm", vocab_size=V, rnn_size=64, num_layers=1), device="cuda",
+                seed=11, dtype="fp32")
+    with torch.no_grad():
+        t.store.flat.mul_(3.0)
+    t.params_changed()
+    s = CharRNN(ModelConfig(model=model, vocab_size=V, rnn_size=H, num_layers=2), device="cuda",
+                seed=1, dtype="fp32")
+    assert t.backend_name == s.backend_name == "native32"
+    x, y = batch(B, T, V, "cuda")
+    d = Teacher(t, top_k=12, alpha=0.7, temperature=2.0).record(x)
+    want, want_state, _ = ReferenceBackend(s.store).train_step(x, y, s.zero_state(B), distill=d)
+    g_ref = s.store.grad[: s.store.numel].clone()
+    loss, state, _ = s.train_step(x, y, s.zero_state(B), distill=d)
+    assert abs(loss.item() - want.item()) < 1e-4 * max(1.0, abs(want.item()))
+    for n in s.store.names():
+        sp = s.store.by_name[n]
+        a, b = (v[sp.offset:sp.offset + sp.numel] for v in (s.store.grad, g_ref))
+        assert ((a - b).norm() / (b.norm() + 1e-12)).item() < 1e-4, n
+    for p, q in zip(state, want_state):
+        for a, b in zip(p, q):
+            assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_teacher_carries_its_state_over_batches(dev):
+    """Two batches in a row against one token at a time from the same start, and the start of an
+    epoch back at zero."""
+    V, B, T, k = 65, 5, 9, 6
+    t, _ = models("lstm", 32, V, dev)
+    x, _ = batch(B, 2 * T, V, dev, seed=3)
+    teacher = Teacher(t, top_k=k, alpha=1.0, temperature=2.0)
+    two = [teacher.record(x[:, :T]), teacher.record(x[:, T:])]
+    st = t.zero_state(B)
+    for i in range(2 * T):
+        logits, st = t.step_logits(x[:, i:i + 1], st)
+        values, _, lse = O.top_logits(logits.float().contiguous(), k, 2.0)
+        d = two[i // T]
+        # (as in test_record_is_time_major)
+        assert torch.allclose(d.values[i % T], values, atol=2e-2, rtol=2e-2), i
+        assert torch.allclose(d.lse[i % T], lse, atol=2e-2, rtol=2e-2), i
+    fresh = Teacher(t, top_k=k, alpha=1.0, temperature=2.0).record(x[:, T:])
+    assert not torch.allclose(fresh.values, two[1].values, atol=2e-2, rtol=2e-2)  # a state mattered
+    teacher.reset(B)
+    again = teacher.record(x[:, :T])
+    assert torch.equal(again.values, two[0].values) and torch.equal(again.lse, two[0].lse)
+
+
+def _rank(rank, world, port, sharded, out_q):
+    import torch.distributed as dist
+
+    from distributed_char_rnn_amd.parallel.grad_sync import GradSync
+    from distributed_char_rnn_amd.parallel.zero import ShardedStep
+
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        t, s = models("lstm", 16, 29, "cpu")
+        opt = TFAdam(s.store, clip=0.5)
+        sync = (ShardedStep(s.store, opt, world, rank) if sharded
+                else GradSync(s.store, world, 8.0, "fp32"))
+        losses = _steps(t, s, opt, lambda v: v[rank * 3:(rank + 1) * 3], sync, sharded)
+        out_q.put((rank, s.store.flat.clone().numpy(), losses))
+    finally:
+        dist.destroy_process_group()
+
+
+def _steps(t, s, opt, rows, sync=None, sharded=False):
+    x, y = batch(6, 24, 29, "cpu", seed=4)
+    x, y = rows(x), rows(y)
+    teacher = Teacher(t, top_k=7, alpha=0.6, temperature=2.0)
+    state, losses = s.zero_state(x.shape[0]), []
+    for i in range(3):
+        part = slice(8 * i, 8 * i + 8)
+        told = teacher.record(x[:, part])
+        if sync is not None:
+            sync.reset()
+        loss, state, _ = s.train_step(x[:, part], y[:, part], state, sync, distill=told)
+        if sharded:
+            sync.step(0.01)
+        else:
+            opt.step(0.01, grad_scale=1.0 if sync is None else sync.finish(defer_scale=True))
+        losses.append(loss.item())
+    return losses
+
+
+@pytest.mark.parametrize("sharded", [False, True])
+def test_two_ranks_with_a_teacher_equal_one_of_twice_the_batch(sharded):
+    """Each rank's teacher reads its own rows and carries their states; replicated and sharded steps
+    end at the parameters of one process with both ranks' rows."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as c:
+        c.bind(("127.0.0.1", 0))
+        port = c.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, 2, port, sharded, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict((r, (flat, losses)) for r, flat, losses in (q.get(timeout=110) for _ in procs))
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    t, s = models("lstm", 16, 29, "cpu")
+    opt = TFAdam(s.store, clip=0.5)
+    losses = _steps(t, s, opt, lambda v: v)
+    np.testing.assert_array_equal(got[0][0], got[1][0])
+    # (as test_distributed.py's cross-entropy steps)
+    np.testing.assert_allclose(got[0][0], s.store.flat.numpy(), rtol=2e-4, atol=2e-6)
+    np.testing.assert_allclose(np.mean([got[0][1], got[1][1]], 0), losses, rtol=1e-5)

@@ -775,3 +775,34 @@ def test_streams_and_graph_replays():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, run()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [300, 20000, 40001, 70001])
+def test_wide_rows_in_a_graph(V, dtype):
+    """The forms of wide rows (large LDS, rows read again), captured: record, loss with its gradient
+    by autograd, draws; each replay with new inputs equals the eager calls."""
+    N, k = 3, 9
+    t, z = rows(N, V, dtype, "cuda", seed=1), rows(N, V, dtype, "cuda", seed=2)
+    u = torch.rand(N, device="cuda")
+
+    def run():
+        v, i, lse = O.top_logits(t, k, 2.0)
+        leaf = z.detach().requires_grad_(True)
+        loss = O.distill_loss(leaf, v, i, top_lse=lse, temperature=2.0)
+        (grad,) = torch.autograd.grad(loss * 3.0, leaf)
+        return (v, i, lse, loss.detach(), grad, O.sample_logits(z, u, top_k=50),
+                O.sample_logits(z, u, top_p=0.9), O.sample_logits(z, u))
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for s in range(3):
+        t.copy_(rows(N, V, dtype, "cuda", seed=10 + s))
+        z.copy_(rows(N, V, dtype, "cuda", seed=20 + s))
+        u.copy_(torch.rand(N, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, run()))
