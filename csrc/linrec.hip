@@ -75,20 +75,14 @@ __device__ __forceinline__ void gates(float f, float& keep, float& take) {
   keep = f >= 0.f ? r : t * r;
   take = f >= 0.f ? t * r : r;
 }
-// The factor of a start, and of every stretch with one: it lets nothing through, not even a NaN.  No
-// product of gates is -0, so a gate or a product that is too small for a number stays apart from it,
-// and a NaN state goes through that.
+// The factor of a stretch with a start: it lets nothing through, not even a NaN.  No product of gates
+// is -0, so a product that is too small for a number stays apart from it, and a NaN state goes through
+// that.  A lane's channels have their starts in common: the first one's factor is asked.
 constexpr float kCut = -0.0f;
 __device__ __forceinline__ bool is_cut(float a) { return __float_as_uint(a) == 0x80000000u; }
-// a h + b
-template <bool MARKS>
-__device__ __forceinline__ float step_(float a, float h, float b) {
-  return MARKS && is_cut(a) ? b : __builtin_fmaf(a, h, b);
-}
-// The factor of two stretches together.
-template <bool MARKS>
-__device__ __forceinline__ float both(float p, float a) {
-  return MARKS && (is_cut(p) || is_cut(a)) ? kCut : p * a;
+// a h + b, or b where the stretch is cut
+__device__ __forceinline__ float step_(bool cut, float a, float h, float b) {
+  return cut ? b : __builtin_fmaf(a, h, b);
 }
 
 struct Lane {  // one lane's VEC channels
@@ -115,9 +109,11 @@ __device__ __forceinline__ void fold_pairs(float (&v)[VEC], const LinrecArgs& p,
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      if (s + i < n)
+      if (s + i < n) {
+        const bool cut = MARKS && is_cut(A[i][0]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = step_<MARKS>(A[i][j], v[j], B[i][j]);
+        for (int j = 0; j < VEC; ++j) v[j] = step_(cut, A[i][j], v[j], B[i][j]);
+      }
   }
 }
 
@@ -159,6 +155,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
   const long BH = (long)p.B * p.H;
 
   float carry[VEC], pa[VEC];  // the state in front of the tile; SUMMARY: the pair so far
+  bool gone = false;          // SUMMARY: a start in it
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
     carry[j] = (!SUMMARY && p.h0) ? p.h0[l.c + j] : 0.f;
@@ -184,15 +181,15 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       const bool live = t0 + i < l.len;
-      const bool start = MARKS && st && st[(long)min(t0 + i, p.T - 1) * p.starts_t];
-      cut |= live && start;
+      const bool start = MARKS && st && live && st[(long)(t0 + i) * p.starts_t];
+      cut |= start;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float keep, take;
         gates(a[i][j], keep, take);
-        a[i][j] = !live ? 1.f : start ? kCut : keep;
+        a[i][j] = start ? kCut : live ? keep : 1.f;
         b[i][j] = live ? take * b[i][j] : 0.f;
-        B[j] = step_<MARKS>(a[i][j], B[j], b[i][j]);
+        B[j] = step_(MARKS && is_cut(a[i][j]), a[i][j], B[j], b[i][j]);
         A[j] *= a[i][j];
       }
     }
@@ -209,21 +206,24 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) h[j] = carry[j];
 #pragma unroll
-    for (int ww = 0; ww < W; ++ww)
+    for (int ww = 0; ww < W; ++ww) {
+      const bool none = MARKS && is_cut(sA[buf][ww][lane * VEC]);
+      gone |= none;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         if (ww == w) h[j] = carry[j];
         const float aa = sA[buf][ww][lane * VEC + j];
-        carry[j] = step_<MARKS>(aa, carry[j], sB[buf][ww][lane * VEC + j]);
-        if (SUMMARY) pa[j] = both<MARKS>(pa[j], aa);
+        carry[j] = step_(none, aa, carry[j], sB[buf][ww][lane * VEC + j]);
+        if (SUMMARY) pa[j] *= aa;
       }
+    }
     if (!SUMMARY) {
 #pragma unroll
       for (int i = 0; i < kC; ++i) {
         float y[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          h[j] = step_<MARKS>(a[i][j], h[j], b[i][j]);
+          h[j] = step_(MARKS && is_cut(a[i][j]), a[i][j], h[j], b[i][j]);
           y[j] = t0 + i < l.len ? h[j] : 0.f;
         }
         if (l.on && t0 + i < p.T) store_row<T, VEC>(out + (long)(t0 + i) * p.h_t, y);
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(64 * W) linrec_fwd_kernel(LinrecArgs p) {
     if (SUMMARY) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        p.sumA[seg * BH + l.c + j] = pa[j];
+        p.sumA[seg * BH + l.c + j] = gone ? kCut : pa[j];
         p.sumB[seg * BH + l.c + j] = carry[j];
       }
     } else if (seg == (int)gridDim.y - 1) {
@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
   const long BH = (long)p.B * p.H;
 
   float e[VEC], pa[VEC];  // the gradient behind the tile; SUMMARY: the pair so far
+  bool gone = false;      // SUMMARY: a start in it
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
     e[j] = (!SUMMARY && p.dlast) ? p.dlast[l.c + j] : 0.f;
@@ -296,9 +297,13 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
         gates(keep[i][j], keep[i][j], take[i][j]);
         if (!live) keep[i][j] = 1.f, take[i][j] = 0.f, g[i][j] = 0.f;
         if (!live && !SUMMARY) xv[i][j] = 0.f;
-        const float a = (MARKS && (cut >> i & 1)) ? kCut : keep[i][j];
-        if (!SUMMARY) B[j] = step_<MARKS>(a, B[j], take[i][j] * xv[i][j]);
-        A[j] *= a;
+        if (SUMMARY) {
+          A[j] *= keep[i][j];
+        } else {
+          const float a = MARKS && (cut >> i & 1) ? kCut : keep[i][j];
+          B[j] = step_(MARKS && is_cut(a), a, B[j], take[i][j] * xv[i][j]);
+          A[j] *= a;
+        }
       }
     }
 #pragma unroll
@@ -316,22 +321,27 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
     if (!SUMMARY)
 #pragma unroll
       for (int ww = 0; ww < W - 1; ++ww)
-        if (ww < w)
+        if (ww < w) {
+          const bool none = MARKS && is_cut(sA[buf][ww][lane * VEC]);
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
-            h[j] = step_<MARKS>(sA[buf][ww][lane * VEC + j], h[j], sB[buf][ww][lane * VEC + j]);
+            h[j] = step_(none, sA[buf][ww][lane * VEC + j], h[j], sB[buf][ww][lane * VEC + j]);
+        }
     float ein[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) ein[j] = e[j];
 #pragma unroll
-    for (int ww = W - 1; ww >= 0; --ww)
+    for (int ww = W - 1; ww >= 0; --ww) {
+      const bool none = MARKS && is_cut(sA[buf][ww][lane * VEC]);
+      gone |= none;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         if (ww == w) ein[j] = e[j];
         const float aa = sA[buf][ww][lane * VEC + j];
-        e[j] = step_<MARKS>(aa, e[j], sG[buf][ww][lane * VEC + j]);
-        if (SUMMARY) pa[j] = both<MARKS>(pa[j], aa);
+        e[j] = step_(none, aa, e[j], sG[buf][ww][lane * VEC + j]);
+        if (SUMMARY) pa[j] *= aa;
       }
+    }
     if (!SUMMARY) {
       float hp[kC][VEC];  // the state that step i multiplies
 #pragma unroll
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(64 * W) linrec_bwd_kernel(LinrecArgs p) {
     if (SUMMARY) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        p.sumA[seg * BH + l.c + j] = pa[j];
+        p.sumA[seg * BH + l.c + j] = gone ? kCut : pa[j];
         p.sumB[seg * BH + l.c + j] = e[j];
       }
     } else if (seg == 0 && p.dh0) {
