@@ -605,7 +605,7 @@ struct LinrecArgs {
   int T, B, H;
   int tiles, tiles_per_seg, segs;  // set by the launcher
 };
-LinrecPlan linrec_plan(int T, int B, int H);
+LinrecPlan linrec_plan(int T, int B, int H, bool is_bf16);
 void launch_linrec(LinrecArgs a, bool is_bf16, bool bwd, hipStream_t s);
 void launch_linrec_step(const LinrecArgs& a, bool is_bf16, hipStream_t s);
 

@@ -438,24 +438,30 @@ void run_type(LinrecArgs& p, bool bwd, int vec, hipStream_t s) {
 
 }  // namespace
 
-// Channels a lane, waves a workgroup and segments of the time axis, from the sizes alone (the
-// backward has to find the forward's tiles).  Measured on one MI355X, forward / backward us:
+// Channels a lane, waves a workgroup and segments of the time axis, from the sizes and the type alone
+// (the backward has to find the forward's tiles).  Measured on one MI355X, launches of a replayed graph
+// over three sets of inputs, forward / backward us:
 //  * the widest loads that leave some 192 workgroups, else single channels: 25600 channels, 1024
-//    steps, bf16: 51 / 68 with two channels a lane, 52 / 78 with one, 108 / 135 with four;
-//  * no more waves than the steps fill (8 steps of 256 x 2048 bf16, both directions: 19 with one, 41
-//    with four); then four waves where a lane has four channels (128 steps of 256 x 512 bf16: 25 / 37,
-//    with eight 25 / 42; 16384 steps of 4 x 1000, padded documents: 165 / 232 against 184 / 275), else
-//    eight: longer tiles, fewer of them (4096 steps of 512 channels: 12.6 / 18.3, with four 14.5 / 21.0);
-//  * segments where even single channels leave fewer workgroups and there are 512 steps or more,
-//    although x, f and dh are then read twice (4096 steps of 512 channels: 12.6 / 18.3 with 64
-//    segments, 41 / 56 with 16); for 200 steps of 6400 channels one segment takes 8.7 / 12.0, eight
-//    11.0 / 12.8.  At most 128 (15390 steps of 384 channels bf16, both directions: 68, with at most
-//    64 78): each workgroup folds the pairs in front of its segment.
-LinrecPlan linrec_plan(int T, int B, int H) {
+//    steps, bf16: 52 / 71 with two channels a lane, 56 / 78 with one, 101 / 124 with four; 12800 channels,
+//    200 steps: 10.1 / 12.9 with one, 12.6 / 16.1 with two;
+//  * no more waves than the steps fill (8 steps of 256 x 2048 bf16: 9.4 / 12.1 with one, 15.5 / 24.9
+//    with four); then four waves where a lane has four channels (128 steps of 256 x 512 bf16: 26 / 42,
+//    with eight 26 / 47; 16384 steps of 4 x 1000, padded documents: 167 / 231 against 180 / 253), else
+//    eight: longer tiles, fewer of them (4096 steps of 512 channels: 13.1 / 20.3, with four 14.9 / 23.8);
+//  * segments where there are few workgroups of single channels and many steps, although x, f and dh
+//    are then read twice (4096 steps of 512 channels: 13.1 / 20.3 with 64 segments, 18 / 35 with 16; 200
+//    steps of 6400 channels: one segment 8.5 / 12.1, four 12.9 / 16.3).  Both directions together, in
+//    segments against one: 512 steps, 48 workgroups 27 against 36 bf16, 26 against 37 fp32; 94: 45
+//    against 39, 37 against 37; 191: 53 against 39, 66 against 51.  768 steps, 94: 51 against 54, 60
+//    against 58; 157: 55 against 54, 79 against 71.  1000 steps, 125: 56 against 69, 82 against 88;
+//    157: 70 against 74, 112 against 93; 191: 81 against 76, 128 against 97.  4096 steps, 125: 181
+//    against 300, 336 against 331; 157: 236 against 307, 438 against 348.  At most 128 (15390 steps of
+//    384 channels bf16: 71, with at most 64 78): each workgroup folds the pairs in front of its segment.
+LinrecPlan linrec_plan(int T, int B, int H, bool is_bf16) {
   LinrecPlan q{};
   auto wgs = [&](int vec) { return ((long)B * (H / vec) + 63) / 64; };
   const int widest = H % 4 == 0 ? 4 : H % 2 == 0 ? 2 : 1;
-  const bool split = T >= 512 && wgs(1) < 192;
+  const bool split = T >= 512 && wgs(1) * 6 < T && wgs(1) < (is_bf16 ? 192 : 128);
   const long cuts = split ? (T / 64 < 128 ? T / 64 : 128) : 1;
   q.vec = widest;
   while (q.vec > 1 && wgs(q.vec) * cuts < (split ? 512 : 192)) q.vec /= 2;
@@ -472,7 +478,7 @@ LinrecPlan linrec_plan(int T, int B, int H) {
 }
 
 void launch_linrec(LinrecArgs p, bool is_bf16, bool bwd, hipStream_t s) {
-  const LinrecPlan q = linrec_plan(p.T, p.B, p.H);
+  const LinrecPlan q = linrec_plan(p.T, p.B, p.H, is_bf16);
   p.tiles = q.tiles;
   p.tiles_per_seg = q.tiles_per_seg;
   p.segs = q.segs;

@@ -2031,7 +2031,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linrec_fwd(
   OnDevice dev(x);
   const auto o = x.options().dtype(at::kFloat);
   at::Tensor h = linrec_out(x), hlast = at::empty({a.B, a.H}, o);
-  const dcr::LinrecPlan q = dcr::linrec_plan(a.T, a.B, a.H);
+  const dcr::LinrecPlan q = dcr::linrec_plan(a.T, a.B, a.H, x.scalar_type() == at::kBFloat16);
   at::Tensor carry = at::empty({want_carry ? q.tiles : 0, a.B, a.H}, o);
   if (a.T == 0 || x.numel() == 0) {
     if (a.h0) hlast.copy_(*h0); else hlast.zero_();
@@ -2055,7 +2055,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linrec_bwd(
   OnDevice dev(x);
   const auto o = x.options().dtype(at::kFloat);
   at::Tensor dx = linrec_out(x), df = linrec_out(f), dh0 = at::empty({a.B, a.H}, o);
-  const dcr::LinrecPlan q = dcr::linrec_plan(a.T, a.B, a.H);
+  const dcr::LinrecPlan q = dcr::linrec_plan(a.T, a.B, a.H, x.scalar_type() == at::kBFloat16);
   check_on(carry, x, at::kFloat, "carry");
   TORCH_CHECK(carry.dim() == 3 && carry.size(0) == q.tiles && carry.size(1) == a.B &&
                   carry.size(2) == a.H && carry.is_contiguous(),
@@ -2500,9 +2500,9 @@ TORCH_LIBRARY(dcr, m) {
         "bool want_carry) -> (Tensor, Tensor, Tensor)");
   m.def("linrec_bwd(Tensor x, Tensor f, Tensor carry, Tensor dh, Tensor? dlast, Tensor? lengths, "
         "Tensor? starts) -> (Tensor, Tensor, Tensor)");
-  m.def("linrec_plan(int T, int B, int H) -> int[]",
-        [](int64_t T, int64_t B, int64_t H) -> std::vector<int64_t> {
-          const dcr::LinrecPlan q = dcr::linrec_plan((int)T, (int)B, (int)H);
+  m.def("linrec_plan(int T, int B, int H, bool bf16) -> int[]",
+        [](int64_t T, int64_t B, int64_t H, bool bf16) -> std::vector<int64_t> {
+          const dcr::LinrecPlan q = dcr::linrec_plan((int)T, (int)B, (int)H, bf16);
           return {q.vec, q.waves, q.tiles, q.segs, q.tiles_per_seg};
         });
   m.def("linrec_step(Tensor x, Tensor f, Tensor(a!) h, Tensor? starts) -> Tensor");

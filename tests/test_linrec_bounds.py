@@ -142,9 +142,9 @@ def test_bounds_hold_and_find_mistakes(which):
     assert "h" in found and "dx" in found and "df" in found
 
 
-def plan(T, B, H):
+def plan(T, B, H, bf16):
     torch.ops.load_library(LIB)
-    return tuple(torch.ops.dcr.linrec_plan(T, B, H))
+    return tuple(torch.ops.dcr.linrec_plan(T, B, H, bf16))
 
 
 @pytest.mark.skipif(not os.path.exists(LIB), reason="native library not built")
@@ -155,9 +155,9 @@ def test_plans_cover_the_steps():
     def size(most):
         return int(torch.exp(torch.rand((), generator=g) * torch.log(torch.tensor(float(most)))))
 
-    for _ in range(3000):
+    for i in range(3000):
         T, B, H = size(1 << 20), size(512), size(4096)
-        vec, waves, tiles, segs, per = plan(T, B, H)
+        vec, waves, tiles, segs, per = plan(T, B, H, i % 2 == 0)
         assert H % vec == 0 and vec in (1, 2, 4) and waves in (1, 2, 4, 8)
         assert waves * vec <= 16
         assert (tiles - 1) * waves * 8 < T <= tiles * waves * 8
@@ -172,8 +172,9 @@ SEGMENTED = [((4500, 3, 1000), (4, 4, 2)), ((9001, 3, 1000), (4, 4, 4)), ((4500,
 
 @pytest.mark.skipif(not os.path.exists(LIB), reason="native library not built")
 @pytest.mark.parametrize("size,want", SEGMENTED)
-def test_segmented_sizes_reach_their_forms(size, want):
-    vec, waves, tiles, segs, per = plan(*size)
+@pytest.mark.parametrize("bf16", [False, True])
+def test_segmented_sizes_reach_their_forms(size, want, bf16):
+    vec, waves, tiles, segs, per = plan(*size, bf16)
     assert (vec, waves, per) == want and segs > 1
     assert tiles % per != 0  # the last segment is short
 
