@@ -12,7 +12,7 @@
 //            + (1 - alpha) (softmax(z)_v - [v = y])
 //
 // One workgroup a row, the row in registers, so z is read once and the gradient written once:
-// that traffic is the bound.  The recorded columns are marked in an LDS bitmap; their threads
+// that traffic is the bound of long fp32 rows, the issue of vector instructions of bf16 ones.  The recorded columns are marked in an LDS bitmap; their threads
 // hold them apart (they write those gradients too), and the rest has a maximum and sum of its
 // own.  So s is never a difference 1 - sum p, which has no digits left where the student is sure.
 //
@@ -65,7 +65,9 @@ __global__ void __launch_bounds__(NT) distill_kernel(DistillArgs a) {
   const bool skip = a.targets && (y < 0 || y >= V);
   const bool ce = a.targets && a.alpha < 1.0f;
   const bool two = ce && inv_t != 1.0f;
-  // x / T - y with one rounding: 1 / T is a sum of two numbers
+  // x / T - y with one rounding: 1 / T is a sum of two numbers.  (For the entries, whose terms are told
+  // apart by d = log(q / p); the columns off them take one rounded log2(e) / T and the exponential of
+  // the hardware: a few units of 2^-24 and |z - max| / T of them.)
   auto scaled = [&](float x, float y) {
     return x == -INFINITY ? x : __builtin_fmaf(x, inv_t, __builtin_fmaf(x, a.inv_t_low, -y));
   };
@@ -289,14 +291,18 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const float* __restri
 
 // Workgroup and registers for N rows of V columns.  One wave takes a row of up to 1024 columns: no
 // barriers, and many rows a CU.  Up to 16384 columns, few rows get more threads, which is faster for
-// the row, and many get smaller workgroups, whose loads and computations overlap each other's
-// (fp32 to bf16, two exponentials: 256 x 8192 8.3 us with 512 threads, 15.6 with 128; 32768 x 8192 359
-// with 128, 401 with 256; 5296 x 12157 bf16 85 with 256, 102 with 512; 21294 x 1897 bf16 80 with 64, 120
-// with 256).  Past 32768 the registers are
-// too few for two workgroups a CU, and a row is read twice instead (1024 x 65536 bf16: 106 us, 121 from
-// registers).  Against the traffic at the rate of a large copy (5.0 TB/s): 32768 x 8192 318 us, 5296 x
-// 12157 51, 2047 x 32001 52 (89 measured: conversions and exponentials of both passes take their
-// share of issue slots beside two workgroups' loads).
+// the row, and many get smaller workgroups, whose loads and computations overlap each other's.
+// Launches of a replayed graph over two or three sets of rows, us, the larger workgroup against the
+// smaller at 256, 512, 1024, 2048 and many rows:
+//   1897 bf16 (256 threads, 64)            6.8  9.7    7.9 10.4   10.9 10.6   17.3 13.1   21294: 118 77
+//   4000 fp32, two exponentials (256, 128) 7.9 10.3   10.0 13.1   15.2 15.1   23.0 22.2    8000: 67 63
+//   8192 fp32 to bf16, two (512, 128)      9.1 16.3   14.5 21.3   22.5 24.6   37.7 38.6   32768: 464 355
+//   12157 bf16 (512, 256)                 10.9 13.4   16.5 17.3   25.6 24.6   44.4 40.4    5296: 101 85
+// (32768 x 8192 with 256 threads: 349.)  Past 32768 the registers are too few for two workgroups a CU,
+// and a row is read twice instead (1024 x 65536 bf16: 99 us, 113 from registers; 2047 x 32001 bf16 112,
+// 92 from registers).  Against the traffic at the rate of a large copy (5.0 TB/s): 32768 x 8192 322 us,
+// 5296 x 12157 51, 21294 x 1897 32, 2047 x 32001 52.  What holds them is the issue of vector instructions:
+// some 40 an element of 64 lanes, the units busy for 93 % of 2047 x 32001 and 98 % of 32768 x 8192.
 template <typename T, typename G>
 static void launch_types(const DistillArgs& a, hipStream_t s) {
   const size_t lds = (size_t)((a.r.V + 31) / 32) * 4;

@@ -19,13 +19,15 @@
 // state in front of every tile (4 / (W kC) bytes per element); the backward recomputes the
 // states of a tile from it in fp32, so it neither reads h nor sees h's rounding to bf16.
 //
-// 128 steps of 256 x 512 bf16: 22 us forward, 33 backward, where the traffic takes 20 and 34 at the
-// rate of a large copy (5.0 TB/s).
+// 128 steps of 256 x 512 bf16: 22 us forward, 33 backward in a kernel trace over one set of inputs, which
+// stays in the last-level cache in part, 26 and 42 over three sets in turn; the traffic takes 20 and 34 at
+// the rate of a large copy (5.0 TB/s).
 //
 // Few channels and many steps leave too few workgroups: the time axis is then cut into
 // segments, a first launch forms each segment's pair, and every workgroup of the second launch
-// folds the pairs in front of its segment, in order, so the result does not depend on timing.
-// 16384 steps of 4 x 1000 bf16 take 386 us so, forward and backward; read once each way 210.
+// folds the pairs in front of its segment, in order, so the result does not depend on timing (every
+// wave of it does, for itself).  16384 steps of 4 x 1000 bf16, padded documents, take some 385 us so, forward
+// and backward; with x, f and dh read once each way the traffic would take 210.
 #include "common.h"
 #include "kernels.h"
 

@@ -8,9 +8,10 @@
 // with k over a quarter of their groups, and rows of many equal values, find the k-th largest
 // value itself by halving a range of values, with counts by ballot.
 //
-// 32768 x 8192 fp32, k = 64: 241 us, 4.5 TB/s (a large copy reaches 5.0); k = 200 398 us, where the
-// places of some 220 entries are the work.  10222 x 864 bf16, k = 31: 20 us; with k = 131, past a
-// quarter of the groups, 78.
+// 32768 x 8192 fp32, k = 64: 241 us, 4.5 TB/s (a large copy reaches 5.0), the vector units busy for 82 %
+// of it; k = 200 359 us, where the places of some 220 entries are the work.  10222 x 864 bf16, k = 31:
+// 21 us of 4 for the read: one wave's chain of reductions a row; with k = 131, past a quarter of the
+// groups, 77.
 #include "vocab_row.h"
 
 namespace dcr {
@@ -106,8 +107,11 @@ __global__ void __launch_bounds__(NT) topk_kernel(RowArgs r, int k, float inv_t,
 }
 
 // One wave takes a row of up to 1024 columns; longer rows get more threads before more registers,
-// and past 65536 columns are read again instead of held (1024 x 65536 bf16, k = 64: 74 us held, 92
-// read again).
+// and past 65536 columns are read again instead of held.  Launches of a replayed graph over three sets of
+// rows, us: 1024 x 65536, k = 64: bf16 71 held, 85 read again; fp32 123 held, although 88 of its registers
+// go to scratch, 154 read again (the read alone takes 27 and 54).  2047 x 32001, k = 32, with 512 threads
+// of 64 columns against 1024 of 32: bf16 50, 61; fp32 100, 94.  5296 x 12157, k = 9, with 512 threads of
+// 32 columns against 256 of 64: bf16 61, 54; fp32 65, 71; 100 rows of it, fp32 8.7, 10.1.
 template <typename T>
 static void launch_type(const RowArgs& r, int k, float inv_t, float* values, int* indices,
                         float* lse, hipStream_t s) {

@@ -11,7 +11,9 @@ it needs no pass over the weights per step: the whole sequence is one or two lau
 ``starts`` (bool ``[T, B]``) marks steps that begin a document: the state restarts there.
 ``lengths`` (int32 ``[B]``, clamped to ``[0, T]``) are the sequences' own lengths in a padded
 batch: behind them output rows are zero, gradients are zero, the padding is never read into a
-result, and the final state is the one after the sequence's last step (``h0`` for length 0).
+result, and the final state is the one after the sequence's last step (``h0`` for length 0).  A
+NaN reaches what depends on it, to its document's last step (backward: its first), and nothing
+else; an infinite state stays one or becomes NaN.
 
 Inputs and outputs are fp32 or bf16; states (``h0``, the final state, their gradients and the
 sums inside) are fp32.  GPU tensors take the HIP kernels (csrc/linrec.hip), CPU tensors the plain
