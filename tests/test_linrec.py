@@ -473,3 +473,26 @@ def test_streams_and_graph_replays():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, both()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,B,H", [(7, 3, 5), (40, 5, 36), (1100, 2, 24)])
+def test_broadcast_inputs(T, B, H, dtype):
+    """Candidates that are the same at every step, gates that are the same in every stream, starts in
+    common: results as of copies, and the gradients of what was broadcast are the sums."""
+    dev = "cuda"
+    x, f, h0, dh, dlast = inputs(T, B, H, dtype, dev)
+    starts = marks(T, 1, "s", dev)[1].expand(T, B)
+    lengths = marks(T, B, "l", dev)[0]
+    v, w = x[0].clone().requires_grad_(True), f[:, :1].clone().requires_grad_(True)
+    xs, fs = v.expand(T, B, H), w.expand(T, B, H)
+    h, last = R.linear_recurrence(xs, fs, h0, lengths=lengths, starts=starts)
+    torch.autograd.backward([h, last], [dh, dlast])
+    a, b = xs.detach().contiguous(), fs.detach().contiguous()
+    want_h, want_last, carry = R.linear_recurrence_fwd(a, b, h0, lengths=lengths,
+                                                       starts=starts.contiguous())
+    assert torch.equal(h, want_h) and torch.equal(last, want_last)
+    dx, df, _ = R.linear_recurrence_bwd(a, b, carry, dh, dlast=dlast, lengths=lengths,
+                                        starts=starts.contiguous())
+    assert torch.equal(v.grad, dx.sum(0)) and torch.equal(w.grad, df.sum(1, keepdim=True))

@@ -196,3 +196,16 @@ def test_segments_against_the_formulas(size, which, dtype):
 def test_forms_against_the_formulas(size, which, dtype):
     args = inputs(*size, dtype, "cuda", which)
     assert misses(run(*args), *formulas(*args)) == []
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [(7, 3, 5), (40, 5, 36), (600, 2, 24)])
+def test_broadcast_inputs_against_the_formulas(size, dtype, dev):
+    """Inputs of stride zero: one step for all, one stream for all.  (On the CPU not bit by bit those of
+    copies: its logistic function of a strided tensor is another of two forms.)"""
+    T, B, H = size
+    x, f, h0, dh, dlast, lengths, starts = inputs(T, B, H, dtype, dev, "ls")
+    args = (x[:1].expand(T, B, H), f[:, :1].expand(T, B, H), h0, dh[:, :1].expand(T, B, H), dlast,
+            lengths, starts[:, :1].expand(T, B))
+    assert misses(run(*args), *formulas(*args)) == []

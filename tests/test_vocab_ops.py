@@ -806,3 +806,29 @@ def test_wide_rows_in_a_graph(V, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, run()))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls in flight on two streams, one row kernel beside another, share nothing."""
+    N, V, k = 300, 9000, 12
+    z = [rows(N, V, F32, "cuda", seed=i) for i in range(2)]
+    u = [torch.rand(N, device="cuda") for _ in range(2)]
+
+    def run(i):
+        v, ix, lse = O.top_logits(z[i], k, 2.0)
+        return (v, ix, lse) + O.distill_xent(z[1 - i], v, ix, top_lse=lse, temperature=2.0) + (
+            O.sample_logits(z[i], u[i], top_p=0.9),)
+
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(side[i]):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
